@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define SMO_ABI_VERSION 3
+#define SMO_ABI_VERSION 4
 
 #if defined(__GNUC__)
 #define SMO_API __attribute__((visibility("default")))
@@ -38,7 +38,8 @@ typedef enum smo_status {
     SMO_ERR_WORKSPACE = 3,   /* workspace missing or smaller than smo_workspace_size() */
     SMO_ERR_CUDA = 4,        /* a CUDA call failed; see smo_last_cuda_error() */
     SMO_ERR_TIMEOUT = 5,     /* a bounded inter-CTA wait gave up (device status) */
-    SMO_ERR_NONFINITE = 6    /* reserved */
+    SMO_ERR_NONFINITE = 6,   /* reserved */
+    SMO_ERR_CAPTURE = 7      /* the stream is capturing and the step's scalars are host values */
 } smo_status;
 
 /* How one tensor's moments are kept (the reference's per-tensor state kinds). */
@@ -205,6 +206,100 @@ SMO_API int smo_pool2d_pair(const float *grad, const float *param, int64_t H, in
  * interpolation of spatial_8bit.py:359-370. */
 SMO_API int smo_upsample2d(const float *src, int64_t h, int64_t w, int64_t H, int64_t W, int64_t interp_band,
                    float *out, void *stream);
+
+/* ---- AdamW over many tensors ------------------------------------------- */
+
+/* How one tensor's AdamW moments are kept. */
+typedef enum smo_adamw_kind {
+    SMO_ADAMW_F32 = 1,       /* exp_avg, exp_avg_sq: fp32, n elements each */
+    SMO_ADAMW_8BIT = 2       /* m_q, m_s, v_q, v_s: codes and block scales */
+} smo_adamw_kind;
+
+/* fp32 scalars of one tensor's AdamW step, each formed in double and rounded once. */
+typedef struct smo_adamw_hyper {
+    float beta1, omb1;       /* beta1, 1 - beta1 */
+    float beta2, omb2;       /* beta2, 1 - beta2 */
+    float decay;             /* 1 - lr * weight_decay (decoupled) */
+    float step_size;         /* lr / (1 - beta1^step) */
+    float rsqrt_bc2;         /* 1 / sqrt(1 - beta2^step) */
+    float eps;
+} smo_adamw_hyper;
+
+/* One parameter tensor of an AdamW step: n consecutive elements of `dtype`
+ * (smo_dtype) in param and grad.  The step, on fp32 numbers, every operation
+ * rounded once:
+ *
+ *   g = scale * grad                                   (scale: see smo_adamw_step)
+ *   m = beta1 * m + omb1 * g;   v = beta2 * v + (omb2 * g) * g
+ *   p = p * decay - (step_size * m) / (sqrt(v) * rsqrt_bc2 + eps)
+ *
+ * p is the fp32 master copy where `master` is given (param then receives its
+ * rounding), else param itself, rounded to dtype when written.
+ *
+ * SMO_ADAMW_8BIT keeps m and u = sqrt(v) in blocks of q_block (64, 128 or 256)
+ * consecutive elements, nb = ceil(n / q_block): one scale a block,
+ * s = max(max |x|, 2^-100), and a code an element that stands for
+ *   m = (c * |c|) * (m_s * (1 / 127^2)),  c in -127..127
+ *   u = (c * c)   * (v_s * (1 / 255^2)),  c in 0..255
+ * c = rint(top * sqrt(|x| * (1 / s))) with x's sign, top = 127 or 255; a
+ * positive u is never stored as 0.  A block that holds a NaN gets the scale
+ * NaN.  m_q, v_q: nb * q_block bytes, 16-byte aligned; the codes behind n are
+ * written as 0.  The update uses m and u before they are coded. */
+typedef struct smo_adamw_tensor {
+    void *param;
+    const void *grad;
+    float *master;           /* NULL: none */
+    float *exp_avg, *exp_avg_sq;
+    int8_t *m_q;
+    float *m_s;
+    uint8_t *v_q;
+    float *v_s;
+    const smo_adamw_hyper *hp_dev;  /* device memory; NULL: hp holds the scalars */
+    int64_t n;
+    int32_t dtype, kind, q_block, reserved;
+    smo_adamw_hyper hp;
+} smo_adamw_tensor;
+
+/* Bytes of device workspace that a step over n tensors with max_norm > 0, or
+ * a gradient norm over n tensors, needs (0 for n <= 0). */
+SMO_API size_t smo_grad_norm_workspace_size(int32_t n);
+
+/* One AdamW step over n tensors, enqueued on `stream`.
+ * grad_scale: a device float that every gradient is multiplied by, or NULL.
+ * max_norm > 0: the gradients are further scaled by min(1, max_norm / (N + 1e-6)),
+ * N = the 2-norm over all of them (after grad_scale); N is written to norm_out (a
+ * device float) if that is not NULL.  The gradients themselves stay as they
+ * are.  workspace: smo_grad_norm_workspace_size(n) bytes, 256-byte aligned,
+ * used only when max_norm > 0 (else NULL, 0). */
+SMO_API int smo_adamw_step(const smo_adamw_tensor *tensors, int32_t n, const float *grad_scale, float max_norm,
+                           float *norm_out, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The moments of SMO_ADAMW_8BIT tensors as 32-bit numbers: exp_avg = m and
+ * exp_avg_sq = u * u receive what the codes stand for (only exp_avg,
+ * exp_avg_sq, the codes, scales, n and q_block are read). */
+SMO_API int smo_adamw_decode(const smo_adamw_tensor *tensors, int32_t n, void *stream);
+
+/* The reverse: codes and scales of exp_avg and sqrt(exp_avg_sq). */
+SMO_API int smo_adamw_encode(const smo_adamw_tensor *tensors, int32_t n, void *stream);
+
+/* sizeof(smo_adamw_tensor) as compiled into the library. */
+SMO_API size_t smo_adamw_tensor_struct_size(void);
+
+/* n consecutive elements of a gradient. */
+typedef struct smo_grad {
+    void *grad;
+    int64_t n;
+    int32_t dtype, reserved;
+} smo_grad;
+
+/* The 2-norm over all elements of n tensors, written to norm_out (a device
+ * float).  Products and sums are held in double and added in an order that
+ * depends on the sizes alone, so the same gradients give the same bits.
+ * max_norm > 0: the tensors are then multiplied in place by
+ * min(1, max_norm / (norm + 1e-6)).  workspace: smo_grad_norm_workspace_size(n)
+ * bytes, 256-byte aligned. */
+SMO_API int smo_grad_norm(const smo_grad *grads, int32_t n, float max_norm, float *norm_out, void *workspace,
+                          size_t workspace_bytes, void *stream);
 
 /* ---- utilities ---------------------------------------------------------- */
 

@@ -106,3 +106,12 @@ def step_scalars(lr, betas, eps, weight_decay, step: int) -> StepScalars:
         neg_step=np.float32(-step_size), sqrt_bc2=np.float32(math.sqrt(bc2)),
         eps=np.float32(eps),
     )
+
+
+def adamw_scalars(lr, betas, eps, weight_decay, step: int):
+    """The scalars of an AdamW step (1-based ``step``), in the order of struct
+    smo_adamw_hyper, formed in double and rounded once to fp32."""
+    lr, beta1, beta2 = float(lr), float(betas[0]), float(betas[1])
+    return tuple(np.float32(x) for x in (
+        beta1, 1 - beta1, beta2, 1 - beta2, 1 - lr * float(weight_decay), lr / (1 - beta1 ** step),
+        1 / math.sqrt(1 - beta2 ** step), float(eps)))

@@ -23,7 +23,10 @@ SMO_DTYPE_F32 = 0
 SMO_DTYPE_BF16 = 1
 SMO_DTYPE_F16 = 2
 SMO_FLAG_GENERAL_PATH = 1
-ABI_VERSION = 3
+SMO_ERR_CAPTURE = 7
+SMO_ADAMW_F32 = 1
+SMO_ADAMW_8BIT = 2
+ABI_VERSION = 4
 
 # Field layout of struct smo_hyper / smo_tensor, as a numpy structured dtype so
 # that descriptor tables are filled column-wise without per-field Python calls.
@@ -47,6 +50,19 @@ TENSOR_DTYPE = np.dtype([
 ])
 
 HYPER_FIELDS = HYPER_DTYPE.names
+
+# struct smo_adamw_hyper / smo_adamw_tensor / smo_grad
+ADAMW_HYPER_DTYPE = np.dtype([(name, np.float32) for name in
+                              ("beta1", "omb1", "beta2", "omb2", "decay", "step_size", "rsqrt_bc2", "eps")])
+
+ADAMW_DTYPE = np.dtype([
+    ("param", np.uint64), ("grad", np.uint64), ("master", np.uint64), ("exp_avg", np.uint64), ("exp_avg_sq", np.uint64),
+    ("m_q", np.uint64), ("m_s", np.uint64), ("v_q", np.uint64), ("v_s", np.uint64), ("hp_dev", np.uint64),
+    ("n", np.int64), ("dtype", np.int32), ("kind", np.int32), ("q_block", np.int32), ("reserved", np.int32),
+    ("hp", ADAMW_HYPER_DTYPE),
+])
+
+GRAD_DTYPE = np.dtype([("grad", np.uint64), ("n", np.int64), ("dtype", np.int32), ("reserved", np.int32)])
 
 
 class SmoError(RuntimeError):
@@ -90,16 +106,26 @@ def load():
         "smo_step_no_alloc": (ctypes.c_int, [P, i32, P, P]),
         "smo_set_wait_limit": (i64, [i64]),
         "smo_inject_wait_timeout": (ctypes.c_int, [ctypes.c_int]),
+        "smo_adamw_step": (ctypes.c_int, [P, i32, P, ctypes.c_float, P, P, sz, P]),
+        "smo_adamw_decode": (ctypes.c_int, [P, i32, P]),
+        "smo_adamw_encode": (ctypes.c_int, [P, i32, P]),
+        "smo_adamw_tensor_struct_size": (sz, []),
+        "smo_grad_norm_workspace_size": (sz, [i32]),
+        "smo_grad_norm": (ctypes.c_int, [P, i32, ctypes.c_float, P, P, sz, P]),
     }
+    lib.smo_abi_version.restype = ctypes.c_int
+    if lib.smo_abi_version() != ABI_VERSION:
+        raise SmoError(f"libsmo_b200 ABI {lib.smo_abi_version()} != binding ABI {ABI_VERSION}")
     for name, (res, args) in sigs.items():
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args
-    if lib.smo_abi_version() != ABI_VERSION:
-        raise SmoError(f"libsmo_b200 ABI {lib.smo_abi_version()} != binding ABI {ABI_VERSION}")
     if lib.smo_tensor_struct_size() != TENSOR_DTYPE.itemsize:
         raise SmoError(f"smo_tensor is {lib.smo_tensor_struct_size()} bytes in the library, "
                        f"{TENSOR_DTYPE.itemsize} in the binding")
+    if lib.smo_adamw_tensor_struct_size() != ADAMW_DTYPE.itemsize:
+        raise SmoError(f"smo_adamw_tensor is {lib.smo_adamw_tensor_struct_size()} bytes in the library, "
+                       f"{ADAMW_DTYPE.itemsize} in the binding")
     _lib = lib
     return lib
 
@@ -120,3 +146,8 @@ def workspace_size(table: np.ndarray) -> int:
 def step(table: np.ndarray, workspace_ptr: int, workspace_bytes: int, stream: int) -> None:
     assert table.dtype == TENSOR_DTYPE and table.flags["C_CONTIGUOUS"]
     check(load().smo_step(table.ctypes.data, len(table), workspace_ptr, workspace_bytes, stream), "smo_step")
+
+
+def address(name: str) -> int:
+    """Address of a library function, for the host extension to call."""
+    return ctypes.cast(getattr(load(), name), ctypes.c_void_p).value

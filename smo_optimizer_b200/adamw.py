@@ -1,0 +1,530 @@
+"""``AdamW`` and ``AdamW8bit``: AdamW with decoupled weight decay over many
+tensors in one launch, and the norm of a set of gradients.
+
+They stand beside ``SMO`` / ``SMO8bit`` for parameters whose moments are kept at
+full resolution: ``AdamW`` holds both moments in fp32 whatever the parameters'
+type, ``AdamW8bit`` in one byte each (square-root companded codes with a scale
+for every block of 64, 128 or 256 elements).  For bf16 and fp16 parameters
+``master_weights=True`` keeps the parameters themselves in fp32 too and hands the
+model their rounding.  The arithmetic is stated in include/smo_b200.h
+(``smo_adamw_tensor``).
+
+As with the other optimizers here the parameters are CUDA tensors (fp32, bf16
+or fp16) with gradients of their own type, the work runs on the current stream,
+and there is no CPU path.
+"""
+
+from __future__ import annotations
+
+from itertools import chain
+
+import numpy as np
+import torch
+from torch.optim.optimizer import Optimizer
+
+from . import _host, _lib
+from .optimizers import _DTYPE_CODES, _host_ext, _named, _same_dense_layout, protected_param_groups
+
+__all__ = ["AdamW", "AdamW8bit", "clip_grad_norm_", "grad_norm"]
+
+BLOCK_SIZES = (64, 128, 256)
+
+_FLOAT_KEYS = ("exp_avg", "exp_avg_sq")
+_CODE_KEYS = ("m_q", "m_s", "v_q", "v_s")
+_STATE_DTYPES = {"exp_avg": torch.float32, "exp_avg_sq": torch.float32, "master": torch.float32, "m_q": torch.int8,
+                 "m_s": torch.float32, "v_q": torch.uint8, "v_s": torch.float32}
+
+
+def _stream(dev) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+# ---------------------------------------------------------------- gradient norms
+
+
+def _gradients(parameters, what):
+    if torch.is_tensor(parameters):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters]
+    grads = [g for g in grads if g is not None]
+    for g in grads:
+        if g.is_sparse:
+            raise RuntimeError(f"{what} does not support sparse gradients.")
+        if g.device.type != "cuda":
+            raise RuntimeError(f"{what} (B200 build) takes CUDA tensors only; got a gradient on {g.device}")
+        if g.dtype not in _DTYPE_CODES:
+            raise TypeError(f"{what} (B200 build) takes fp32, bf16 or fp16 gradients; got {g.dtype}")
+        if g.device != grads[0].device:
+            raise RuntimeError(f"{what} takes the gradients of one device; got {grads[0].device} and {g.device}")
+    return grads
+
+
+def _norm(grads, max_norm, what):
+    lib = _lib.load()
+    ext, fn, ws = _host_ext(), _lib.address("smo_grad_norm"), _lib.address("smo_grad_norm_workspace_size")
+    got = ext.grad_norm(grads, max_norm, fn, ws)
+    if got is None:
+        # gradients with gaps or repeated elements: on copies, written back when clipped
+        copies = [g.contiguous() for g in grads]
+        got = ext.grad_norm(copies, max_norm, fn, ws)
+        if max_norm > 0:
+            for g, c in zip(grads, copies):
+                if c is not g:
+                    g.copy_(c)
+    _lib.check(got[0], what)
+    return got[1]
+
+
+@torch.no_grad()
+def grad_norm(parameters) -> torch.Tensor:
+    """The 2-norm over the gradients of all ``parameters`` (an iterable, or one
+    parameter) as one vector: an fp32 tensor of no dimensions on their device.
+
+    Parameters without a gradient are left out.  Each gradient is read once;
+    squares and sums are held in double, in an order that depends on the sizes
+    alone, so the same gradients always give the same bits.  Nothing
+    synchronises."""
+    grads = _gradients(parameters, "grad_norm")
+    if not grads:
+        return torch.zeros(())
+    return _norm(grads, 0.0, "grad_norm")
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
+    """Multiplies the gradients of all ``parameters`` in place by
+    ``min(1, max_norm / (norm + 1e-6))`` and returns ``norm``, their 2-norm before
+    (see ``grad_norm``).  A norm that is NaN makes every gradient NaN.
+
+    ``AdamW`` and ``AdamW8bit`` clip within the step (``max_grad_norm``), without
+    writing the gradients; this is for ``SMO``, ``SMO8bit`` and any other user of
+    the gradients."""
+    max_norm = float(max_norm)
+    if not max_norm > 0.0:
+        raise ValueError(f"Invalid max_norm: {max_norm}")
+    grads = _gradients(parameters, "clip_grad_norm_")
+    if not grads:
+        return torch.zeros(())
+    return _norm(grads, max_norm, "clip_grad_norm_")
+
+
+# ---------------------------------------------------------------- optimizers
+
+
+class _AdamWBase(Optimizer):
+    _name = "AdamW"
+
+    def __init__(self, params, lr, betas, eps, weight_decay, master_weights, max_grad_norm, extra):
+        if not 0.0 <= lr:
+            raise ValueError(f"Invalid learning rate: {lr}")
+        if not 0.0 <= eps:
+            raise ValueError(f"Invalid epsilon value: {eps}")
+        if not 0.0 <= betas[0] < 1.0:
+            raise ValueError(f"Invalid beta parameter at index 0: {betas[0]}")
+        if not 0.0 <= betas[1] < 1.0:
+            raise ValueError(f"Invalid beta parameter at index 1: {betas[1]}")
+        if not 0.0 <= weight_decay:
+            raise ValueError(f"Invalid weight_decay value: {weight_decay}")
+        if max_grad_norm is not None and not max_grad_norm > 0.0:
+            raise ValueError(f"Invalid max_grad_norm: {max_grad_norm}")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, **extra))
+        self.master_weights = bool(master_weights)
+        self.max_grad_norm = max_grad_norm
+        # norm of the gradients that the last step saw, before clipping; kept
+        # only with max_grad_norm, and overwritten by the next step
+        self.last_grad_norm = None
+        self._plan = None       # (capsule of the C++ host path, device index, number of tensors)
+        self._workspace = {}    # device index -> (workspace, norm)
+
+    # ---------------------------------------------------------------- state
+
+    # torch's Optimizer pickles (and deep-copies) its groups and state only
+    _SETTINGS = ("master_weights", "max_grad_norm")
+
+    def __getstate__(self):
+        return dict(super().__getstate__(), **{k: getattr(self, k) for k in self._SETTINGS})
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._plan = None
+        self._workspace = {}
+        self.last_grad_norm = None
+
+    def _eight_bit(self, p, group) -> bool:
+        return False
+
+    def _init_state(self, p, group):
+        state = self.state[p]
+        state["step"] = 0
+        if self._eight_bit(p, group):
+            block = group["block_size"]
+            nb = _host.num_blocks(p.numel(), block)
+            for q, s, dtype in (("m_q", "m_s", torch.int8), ("v_q", "v_s", torch.uint8)):
+                state[q] = torch.zeros((nb, block), dtype=dtype, device=p.device)
+                state[s] = torch.zeros((nb, 1), dtype=torch.float32, device=p.device)
+        else:
+            for key in _FLOAT_KEYS:
+                state[key] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+
+    def _ready(self):
+        """Checks every parameter with a gradient and gives it its state."""
+        found = []
+        for group in self.param_groups:
+            for p in group["params"]:
+                grad = p.grad
+                if grad is None:
+                    continue
+                if grad.is_sparse:
+                    raise RuntimeError(f"{self._name} does not support sparse gradients.")
+                if p.device.type != "cuda":
+                    raise RuntimeError(f"{self._name} (B200 build) steps CUDA tensors only; "
+                                       f"got a parameter on {p.device}")
+                if p.dtype not in _DTYPE_CODES or grad.dtype != p.dtype:
+                    raise TypeError(f"{self._name} (B200 build) steps fp32, bf16 or fp16 parameters with "
+                                    f"gradients of the same dtype; got {p.dtype} / {grad.dtype}")
+                state = self.state[p]
+                if "step" not in state:
+                    self._init_state(p, group)
+                if self.master_weights and p.dtype != torch.float32 and "master" not in state:
+                    state["master"] = p.detach().to(torch.float32, memory_format=torch.preserve_format)
+                found.append((p, grad, state, group))
+        return found
+
+    def load_state_dict(self, state_dict):
+        """Loads what ``state_dict()`` of this class, of the other one here or of
+        ``torch.optim.AdamW`` returned: moments are kept in 32 bits, and brought
+        into 8 bits or out of them (or to another block size) where this
+        optimizer holds them so."""
+        last = {}
+        # registered last: sees the dict as the other hooks leave it
+        hook = self.register_load_state_dict_pre_hook(lambda opt, sd: last.update(sd))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            hook.remove()
+        for group in self.param_groups:
+            for key, value in self.defaults.items():
+                group.setdefault(key, value)
+        names = chain.from_iterable(g["params"] for g in last["param_groups"])
+        own = ((p, g) for g in self.param_groups for p in g["params"])
+        for name, (p, group) in zip(names, own):
+            saved = last["state"].get(name)
+            if not saved:
+                continue
+            # torch's loader has cast every tensor to the parameter's type: take the saved ones
+            state = {"step": int(saved.get("step", 0))}
+            for key, dtype in _STATE_DTYPES.items():
+                if torch.is_tensor(saved.get(key)):
+                    state[key] = saved[key].to(device=p.device, dtype=dtype)
+            if not self.master_weights or p.dtype == torch.float32:
+                state.pop("master", None)
+            self.state[p] = self._adopt(p, state, group)
+
+    def _adopt(self, p, state, group):
+        """A loaded state as this optimizer holds it."""
+        shape = tuple(p.shape)
+        for key in _FLOAT_KEYS + ("master",):
+            if key in state and tuple(state[key].shape) != shape:
+                raise ValueError(f"state['{key}'] has the shape {tuple(state[key].shape)}; the parameter's is {shape}")
+        coded = all(k in state for k in _CODE_KEYS)
+        if coded:
+            q = state["m_q"]
+            block = q.shape[1] if q.dim() == 2 else 0
+            nb = _host.num_blocks(p.numel(), block) if block in BLOCK_SIZES else -1
+            for key in _CODE_KEYS:
+                want = (nb, block) if key.endswith("_q") else (nb, 1)
+                if tuple(state[key].shape) != want:
+                    raise ValueError(f"state['{key}'] has the shape {tuple(state[key].shape)}, which no block size of "
+                                     f"{BLOCK_SIZES} gives a parameter of {p.numel()} elements")
+                state[key] = state[key].contiguous()
+        elif not all(k in state for k in _FLOAT_KEYS):
+            raise ValueError("the loaded state has neither exp_avg and exp_avg_sq nor m_q, m_s, v_q and v_s")
+        eight = self._eight_bit(p, group)
+        if coded and not (eight and group["block_size"] == block):
+            state.update(zip(_FLOAT_KEYS, _decode([(p, state)])[0]))
+            coded = False
+            for key in _CODE_KEYS:
+                del state[key]
+        if eight and not coded:
+            state.update(_encode(p, state, group["block_size"]))
+            for key in _FLOAT_KEYS:
+                del state[key]
+        return state
+
+    # ---------------------------------------------------------------- step
+
+    def step(self, closure=None, grad_scale=None):
+        """One step of every parameter that has a gradient.
+
+        ``grad_scale``: an fp32 tensor of one element on the parameters' device;
+        the step multiplies every gradient by it (and leaves the gradients as
+        they are).  ``max_grad_norm`` bounds the scaled gradients' norm."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if grad_scale is not None:
+            if not torch.is_tensor(grad_scale) or grad_scale.dtype != torch.float32 or grad_scale.numel() != 1:
+                raise TypeError("grad_scale must be an fp32 tensor of one element")
+        if self._plan is not None:
+            rc = self._run_plan(grad_scale)
+            if rc >= 0:
+                return loss
+        with torch.no_grad():
+            items = self._ready()
+            self._plan = None
+            if not items:
+                self.last_grad_norm = None
+                return loss
+            self._plan = _host_ext().adamw_plan(self.param_groups, self.state, _lib.address("smo_adamw_step"))
+            if self._plan is None or self._run_plan(grad_scale) < 0:
+                self._plan = None
+                self._slow_step(items, grad_scale)
+        return loss
+
+    def _scale_address(self, grad_scale, index):
+        if grad_scale is None:
+            return 0
+        if grad_scale.device.type != "cuda" or grad_scale.device.index != index:
+            raise RuntimeError(f"grad_scale must be on the parameters' device (cuda:{index}); got {grad_scale.device}")
+        return grad_scale.data_ptr()
+
+    def _norm_buffers(self, index, tensors):
+        """(max_norm, norm address, workspace address, bytes) of a step over so many tensors of a device."""
+        if self.max_grad_norm is None:
+            self.last_grad_norm = None
+            return 0.0, 0, 0, 0
+        need = _lib.load().smo_grad_norm_workspace_size(tensors)
+        kept = self._workspace.get(index)
+        if kept is None or kept[0].numel() < need:
+            dev = torch.device("cuda", index)
+            kept = (torch.empty(need, dtype=torch.uint8, device=dev), torch.zeros((), device=dev))
+            self._workspace[index] = kept
+        self.last_grad_norm = kept[1]
+        return float(self.max_grad_norm), kept[1].data_ptr(), kept[0].data_ptr(), kept[0].numel()
+
+    def _run_plan(self, grad_scale) -> int:
+        cap, index, tensors = self._plan
+        scale = self._scale_address(grad_scale, index)
+        rc = _host_ext().adamw_run(cap, scale, *self._norm_buffers(index, tensors))
+        if rc > 0:
+            self._check(rc)
+        return rc
+
+    def _check(self, rc):
+        if rc == _lib.SMO_ERR_CAPTURE:
+            raise RuntimeError(f"{self._name}.step cannot be captured into a CUDA graph: the step count and the learning "
+                               "rate are host values, which every replay would repeat")
+        _lib.check(rc, "smo_adamw_step")
+
+    def _slow_step(self, items, grad_scale):
+        """Several devices, or parameters, gradients or moments that do not share
+        one layout: the latter are stepped on contiguous copies, written back in
+        stream order."""
+        per_dev = {}
+        for item in items:
+            per_dev.setdefault(item[0].device, []).append(item)
+        if len(per_dev) > 1 and (self.max_grad_norm is not None or grad_scale is not None):
+            raise RuntimeError(f"{self._name}: max_grad_norm and grad_scale need all parameters on one device")
+        for dev, items in per_dev.items():
+            table = np.zeros(len(items), dtype=_lib.ADAMW_DTYPE)
+            back, keep = [], []
+            for rec, (p, grad, state, group) in zip(table, items):
+                self._fill(rec, p, grad, state, group, back, keep)
+            with torch.cuda.device(dev):
+                scale = self._scale_address(grad_scale, dev.index)
+                max_norm, norm, ws, nbytes = self._norm_buffers(dev.index, len(items))
+                self._check(_lib.load().smo_adamw_step(table.ctypes.data, len(table), scale, max_norm, norm, ws, nbytes,
+                                                       _stream(dev)))
+                for dst, src in back:
+                    dst.copy_(src)
+            for p, grad, state, group in items:
+                state["step"] += 1
+
+    @staticmethod
+    def _fill(rec, p, grad, state, group, back, keep):
+        coded = all(k in state for k in _CODE_KEYS)
+        floats = ("master",) if "master" in state else ()
+        floats += () if coded else _FLOAT_KEYS
+        for key in floats + (_CODE_KEYS if coded else ()):
+            t = state.get(key)
+            if not torch.is_tensor(t) or t.dtype != _STATE_DTYPES[key] or t.device != p.device:
+                raise TypeError(f"state['{key}'] must be a {_STATE_DTYPES[key]} tensor on {p.device}")
+            if key in floats and t.shape != p.shape:
+                raise ValueError(f"state['{key}'] must have the parameter's shape {tuple(p.shape)}")
+        held = {k: state[k] for k in floats}
+        direct = _same_dense_layout(p, *held.values()) and (not coded or p.is_contiguous())
+
+        def local(t, out):
+            # the tensor itself, or a contiguous copy of it that is written back
+            if direct or t.is_contiguous():
+                return t
+            c = t.contiguous()
+            keep.append(c)
+            if out:
+                back.append((t, c))
+            return c
+
+        if direct:
+            g = grad
+            if grad.shape != p.shape or grad.stride() != p.stride():
+                g = torch.empty_like(p).copy_(grad)  # empty_like keeps the dense layout of p
+        else:
+            g = grad.contiguous()
+        keep.append(g)
+        rec["param"], rec["grad"] = local(p.detach(), True).data_ptr(), g.data_ptr()
+        for k, t in held.items():
+            rec[k] = local(t, True).data_ptr()
+        rec["n"], rec["dtype"] = p.numel(), _DTYPE_CODES[p.dtype]
+        if coded:
+            block = state["m_q"].shape[-1]
+            nb = _host.num_blocks(p.numel(), block) if block in BLOCK_SIZES else -1
+            for k in _CODE_KEYS:
+                t = state[k]
+                if t.numel() != (nb * block if k.endswith("_q") else nb) or not t.is_contiguous():
+                    raise ValueError(f"state['{k}'] must be contiguous, with a block size of {BLOCK_SIZES}")
+                rec[k] = t.data_ptr()
+            rec["kind"], rec["q_block"] = _lib.SMO_ADAMW_8BIT, block
+        else:
+            rec["kind"] = _lib.SMO_ADAMW_F32
+        rec["hp"] = _host.adamw_scalars(group["lr"], group["betas"], group["eps"], group["weight_decay"],
+                                        state["step"] + 1)
+
+
+class AdamW(_AdamWBase):
+    """AdamW (decoupled weight decay), both moments in fp32.
+
+    ``master_weights``: keep an fp32 copy of each bf16 or fp16 parameter
+    (``state[p]["master"]``), step that, and write its rounding to the parameter.
+    The copy is made of the parameter at its first step; a parameter that is
+    changed from outside afterwards needs its copy changed too.
+    ``max_grad_norm``: scale the gradients of each step by
+    ``min(1, max_grad_norm / (norm + 1e-6))`` within the step;
+    ``last_grad_norm`` is then the norm (a device tensor, overwritten by the next
+    step).
+
+    ``state[p]``: ``step`` (int), ``exp_avg``, ``exp_avg_sq``, with master weights
+    ``master``."""
+    _name = "AdamW"
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, master_weights=False,
+                 max_grad_norm=None):
+        super().__init__(params, lr, betas, eps, weight_decay, master_weights, max_grad_norm, {})
+
+
+class AdamW8bit(_AdamWBase):
+    """AdamW with moments of one byte an element.
+
+    The first moment m and u, the root of the second, are kept in blocks of
+    ``block_size`` (64, 128 or 256) consecutive elements as codes ``c`` that stand
+    for ``s * sign(c) * (c / 127)**2`` and ``s * (c / 255)**2``, ``s`` the block's
+    largest value: relative steps of 2 / c, so the larger values, which steer the
+    update, are held most finely.  The update itself uses the moments before they
+    are coded.  Codes round to the nearest, so a moment that changes by less than
+    half its step between two updates keeps its code: as with other moments of
+    8 bits, a slow drift of a small second moment is followed late.
+
+    Tensors of fewer than ``min_8bit_numel`` elements, and those of groups with
+    ``compress=False``, keep fp32 moments as in ``AdamW``; ``protect_output``
+    makes such groups by the parameters' names, as for ``SMO8bit``.
+
+    ``state[p]``: ``step``, ``m_q`` (int8) and ``v_q`` (uint8) of shape
+    (blocks, block_size), ``m_s`` and ``v_s`` (fp32) of shape (blocks, 1)."""
+    _name = "AdamW8bit"
+    _SETTINGS = _AdamWBase._SETTINGS + ("min_8bit_numel",)
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, block_size=128,
+                 min_8bit_numel=4096, master_weights=False, max_grad_norm=None, protect_output=False):
+        if block_size not in BLOCK_SIZES:
+            raise ValueError(f"Invalid block_size: {block_size}. Must be one of {BLOCK_SIZES}")
+        if not 0 <= min_8bit_numel:
+            raise ValueError(f"Invalid min_8bit_numel: {min_8bit_numel}")
+        if protect_output:
+            params = protected_param_groups(_named(params), protect_output)
+        self.min_8bit_numel = int(min_8bit_numel)
+        super().__init__(params, lr, betas, eps, weight_decay, master_weights, max_grad_norm,
+                         dict(block_size=block_size))
+
+    def _eight_bit(self, p, group) -> bool:
+        return bool(group.get("compress", True)) and p.numel() >= max(1, self.min_8bit_numel)
+
+    @torch.no_grad()
+    def moments(self, params=None, out=None):
+        """``[(exp_avg, exp_avg_sq)]`` of ``params`` (default: every parameter
+        that has a state) as fp32 tensors of the parameters' shapes: what the
+        codes stand for, all tensors in one launch.  A parameter whose moments
+        are kept in fp32 gives those.  ``out``: pairs of contiguous fp32 tensors
+        to write to."""
+        if params is None:
+            params = [p for g in self.param_groups for p in g["params"] if self.state.get(p)]
+        params = [params] if torch.is_tensor(params) else list(params)
+        if out is not None:
+            out = list(out)
+            got = _host_ext().adamw_moments(self.state, params, out, _lib.address("smo_adamw_decode"))
+            if got >= 0:
+                _lib.check(got, "smo_adamw_decode")
+                return out
+            if len(out) != len(params):
+                raise ValueError(f"{len(params)} parameters, {len(out)} outputs")
+        for p in params:
+            if not self.state.get(p):
+                raise KeyError("moments of a parameter that has no state yet")
+        coded = [i for i, p in enumerate(params) if "m_q" in self.state[p]]
+        pairs = [None if "m_q" in self.state[p] else tuple(self.state[p][k] for k in _FLOAT_KEYS) for p in params]
+        if out is None:
+            for i, pair in zip(coded, _decode([(params[i], self.state[params[i]]) for i in coded])):
+                pairs[i] = pair
+            return pairs
+        for p, pair in zip(params, out):
+            for t in pair:
+                if t.dtype != torch.float32 or t.device != p.device or t.shape != p.shape or not t.is_contiguous():
+                    raise TypeError(f"out must be contiguous fp32 tensors of the parameters' shapes on {p.device}")
+        _decode([(params[i], self.state[params[i]]) for i in coded], [out[i] for i in coded])
+        for pair, dst in zip(pairs, out):
+            if pair is not None:
+                for d, s in zip(dst, pair):
+                    d.copy_(s)
+        return out
+
+
+def _coded_row(rec, p, state):
+    block = state["m_q"].shape[1]
+    rec["kind"], rec["q_block"], rec["n"] = _lib.SMO_ADAMW_8BIT, block, p.numel()
+    for k in _CODE_KEYS:
+        rec[k] = state[k].data_ptr()
+
+
+def _launch_codes(name, rows):
+    """smo_adamw_decode / smo_adamw_encode over [(p, state, exp_avg, exp_avg_sq)], one call a device."""
+    per_dev = {}
+    for row in rows:
+        if row[0].device.type != "cuda":
+            raise RuntimeError(f"8-bit moments (B200 build) are kept on CUDA devices only; got {row[0].device}")
+        per_dev.setdefault(row[0].device, []).append(row)
+    for dev, rows in per_dev.items():
+        table = np.zeros(len(rows), dtype=_lib.ADAMW_DTYPE)
+        for rec, (p, state, m, v) in zip(table, rows):
+            _coded_row(rec, p, state)
+            rec["exp_avg"], rec["exp_avg_sq"] = m.data_ptr(), v.data_ptr()
+        with torch.cuda.device(dev):
+            _lib.check(getattr(_lib.load(), name)(table.ctypes.data, len(table), _stream(dev)), name)
+
+
+def _decode(items, out=None):
+    """fp32 moments of [(p, state)] with codes."""
+    if out is None:
+        out = [tuple(torch.empty(p.shape, dtype=torch.float32, device=p.device) for _ in range(2)) for p, _ in items]
+    _launch_codes("smo_adamw_decode", [(p, st, m, v) for (p, st), (m, v) in zip(items, out)])
+    return out
+
+
+def _encode(p, state, block):
+    """Codes and scales of a state's exp_avg and exp_avg_sq."""
+    nb = _host.num_blocks(p.numel(), block)
+    got = {}
+    for q, s, dtype in (("m_q", "m_s", torch.int8), ("v_q", "v_s", torch.uint8)):
+        got[q] = torch.zeros((nb, block), dtype=dtype, device=p.device)
+        got[s] = torch.zeros((nb, 1), dtype=torch.float32, device=p.device)
+    m, v = state["exp_avg"].contiguous(), state["exp_avg_sq"].contiguous()
+    _launch_codes("smo_adamw_encode", [(p, got, m, v)])
+    return got

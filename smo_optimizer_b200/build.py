@@ -9,8 +9,8 @@ cross-compiles.  ``-fmad=false`` keeps every multiply and add separately
 rounded unless the source asks for a fused multiply-add explicitly; the fp32
 op order must match the reference bit for bit.
 
-``csrc/smo_host.cpp`` (the per-step host work of the optimizer classes) is a
-CPython extension compiled with g++ against the installed torch's headers and
+``csrc/smo_host.cpp`` and ``csrc/adamw_host.cpp`` (the per-step host work of the
+optimizer classes) are one CPython extension compiled with g++ against the installed torch's headers and
 libraries; it calls the CUDA library through a function pointer handed over
 by the binding, so both use the one library ctypes loaded.
 """
@@ -97,7 +97,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB_PATH
 
 
-HOST_SRC = os.path.join(CSRC, "smo_host.cpp")
+HOST_SRCS = [os.path.join(CSRC, f) for f in ("smo_host.cpp", "adamw_host.cpp")]
 
 
 def host_ext_path() -> str:
@@ -112,7 +112,7 @@ def build_host(force: bool = False, verbose: bool = False) -> str:
     import torch
 
     out = host_ext_path()
-    srcs = [HOST_SRC, os.path.join(INCLUDE, "smo_b200.h")]
+    srcs = [*HOST_SRCS, os.path.join(CSRC, "smo_host.h"), os.path.join(INCLUDE, "smo_b200.h")]
     if not force and os.path.exists(out) and all(os.path.getmtime(d) <= os.path.getmtime(out) for d in srcs):
         return out
     cuda_home = os.path.dirname(os.path.dirname(nvcc_path()))
@@ -122,7 +122,7 @@ def build_host(force: bool = False, verbose: bool = False) -> str:
     libdirs = [os.path.join(torch_dir, "lib")]
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *[f"-I{d}" for d in incs], HOST_SRC, "-o", out + ".tmp",
+           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *[f"-I{d}" for d in incs], *HOST_SRCS, "-o", out + ".tmp",
            *[f"-L{d}" for d in libdirs], *[f"-Wl,-rpath,{d}" for d in libdirs],
            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
     if verbose:

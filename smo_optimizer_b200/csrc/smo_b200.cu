@@ -824,6 +824,7 @@ const char *smo_status_string(int status) {
         case SMO_ERR_CUDA: return "CUDA error";
         case SMO_ERR_TIMEOUT: return "bounded device wait timed out";
         case SMO_ERR_NONFINITE: return "non-finite value";
+        case SMO_ERR_CAPTURE: return "stream capture of a step whose scalars are host values";
         default: return "unknown status";
     }
 }

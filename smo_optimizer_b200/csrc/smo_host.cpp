@@ -34,14 +34,51 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "smo_b200.h"
+#include "smo_host.h"
 
-namespace {
-
-using StepFn = int (*)(const smo_tensor *, int32_t, void *, size_t, void *);
+namespace smo_host {
 
 PyObject *s_params, *s_step, *s_lr, *s_betas, *s_eps, *s_weight_decay;
 int g_watcher = -1;
 unsigned long long g_state_generation = 0;  // bumped on any change to a watched state mapping
+
+}  // namespace smo_host
+
+using namespace smo_host;
+
+bool smo_host::read_group(PyObject *g, double *out) {
+    PyObject *lr = PyDict_GetItemWithError(g, s_lr);
+    PyObject *betas = PyDict_GetItemWithError(g, s_betas);
+    PyObject *eps = PyDict_GetItemWithError(g, s_eps);
+    PyObject *wd = PyDict_GetItemWithError(g, s_weight_decay);
+    if (!lr || !betas || !eps || !wd) return false;
+    PyObject *b0, *b1;
+    if (PyTuple_Check(betas) && PyTuple_GET_SIZE(betas) == 2) {
+        b0 = PyTuple_GET_ITEM(betas, 0);
+        b1 = PyTuple_GET_ITEM(betas, 1);
+    } else if (PyList_Check(betas) && PyList_GET_SIZE(betas) == 2) {
+        b0 = PyList_GET_ITEM(betas, 0);
+        b1 = PyList_GET_ITEM(betas, 1);
+    } else {
+        return false;
+    }
+    // plain numbers only (a tensor-valued hyperparameter takes the Python path)
+    if (!PyFloat_Check(lr) && !PyLong_Check(lr)) return false;
+    if (!PyFloat_Check(b0) && !PyLong_Check(b0)) return false;
+    if (!PyFloat_Check(b1) && !PyLong_Check(b1)) return false;
+    if (!PyFloat_Check(eps) && !PyLong_Check(eps)) return false;
+    if (!PyFloat_Check(wd) && !PyLong_Check(wd)) return false;
+    out[0] = PyFloat_AsDouble(lr);
+    out[1] = PyFloat_AsDouble(b0);
+    out[2] = PyFloat_AsDouble(b1);
+    out[3] = PyFloat_AsDouble(eps);
+    out[4] = PyFloat_AsDouble(wd);
+    return !PyErr_Occurred();
+}
+
+namespace {
+
+using StepFn = int (*)(const smo_tensor *, int32_t, void *, size_t, void *);
 
 int on_state_change(PyDict_WatchEvent, PyObject *, PyObject *, PyObject *) {
     g_state_generation++;
@@ -119,37 +156,6 @@ smo_hyper make_hyper(const double *in, long long step) {
     h.sqrt_bc2 = (float)std::sqrt(bc2);
     h.eps = (float)eps;
     return h;
-}
-
-// a group's lr, betas, eps and weight_decay as doubles (false: not numbers)
-bool read_group(PyObject *g, double *out) {
-    PyObject *lr = PyDict_GetItemWithError(g, s_lr);
-    PyObject *betas = PyDict_GetItemWithError(g, s_betas);
-    PyObject *eps = PyDict_GetItemWithError(g, s_eps);
-    PyObject *wd = PyDict_GetItemWithError(g, s_weight_decay);
-    if (!lr || !betas || !eps || !wd) return false;
-    PyObject *b0, *b1;
-    if (PyTuple_Check(betas) && PyTuple_GET_SIZE(betas) == 2) {
-        b0 = PyTuple_GET_ITEM(betas, 0);
-        b1 = PyTuple_GET_ITEM(betas, 1);
-    } else if (PyList_Check(betas) && PyList_GET_SIZE(betas) == 2) {
-        b0 = PyList_GET_ITEM(betas, 0);
-        b1 = PyList_GET_ITEM(betas, 1);
-    } else {
-        return false;
-    }
-    // plain numbers only (a tensor-valued hyperparameter takes the Python path)
-    if (!PyFloat_Check(lr) && !PyLong_Check(lr)) return false;
-    if (!PyFloat_Check(b0) && !PyLong_Check(b0)) return false;
-    if (!PyFloat_Check(b1) && !PyLong_Check(b1)) return false;
-    if (!PyFloat_Check(eps) && !PyLong_Check(eps)) return false;
-    if (!PyFloat_Check(wd) && !PyLong_Check(wd)) return false;
-    out[0] = PyFloat_AsDouble(lr);
-    out[1] = PyFloat_AsDouble(b0);
-    out[2] = PyFloat_AsDouble(b1);
-    out[3] = PyFloat_AsDouble(eps);
-    out[4] = PyFloat_AsDouble(wd);
-    return !PyErr_Occurred();
 }
 
 // -1: the plan does not apply (nothing modified); 0: stepped; > 0: smo_status
@@ -390,6 +396,12 @@ PyMethodDef methods[] = {
     {"plan_new", plan_new, METH_VARARGS, "Build a step plan (see smo_host.cpp)."},
     {"plan_step", plan_step, METH_O, "Run one step of a plan: 0, -1 (plan does not apply) or an smo_status."},
     {"hyper_bytes", hyper_bytes, METH_VARARGS, "smo_hyper bytes of (lr, beta1, beta2, eps, weight_decay, step)."},
+    {"adamw_plan", adamw_plan, METH_VARARGS, "Build an AdamW step plan, or None (see adamw_host.cpp)."},
+    {"adamw_run", adamw_run, METH_VARARGS, "Run one step of an AdamW plan: 0, -1 (it does not apply) or an smo_status."},
+    {"adamw_hyper_bytes", adamw_hyper_bytes, METH_VARARGS,
+     "smo_adamw_hyper bytes of (lr, beta1, beta2, eps, weight_decay, step)."},
+    {"adamw_moments", adamw_moments, METH_VARARGS, "8-bit moments as 32-bit numbers: 0, -1 or an smo_status."},
+    {"grad_norm", grad_norm, METH_VARARGS, "Norm of all gradients, or None where one needs a copy."},
     {nullptr, nullptr, 0, nullptr},
 };
 
@@ -404,10 +416,11 @@ PyMODINIT_FUNC PyInit__smo_host(void) {
     s_betas = PyUnicode_InternFromString("betas");
     s_eps = PyUnicode_InternFromString("eps");
     s_weight_decay = PyUnicode_InternFromString("weight_decay");
-    if (!s_params || !s_step || !s_lr || !s_betas || !s_eps || !s_weight_decay) return nullptr;
+    if (!s_params || !s_step || !s_lr || !s_betas || !s_eps || !s_weight_decay || !adamw_init()) return nullptr;
     g_watcher = PyDict_AddWatcher(on_state_change);
     if (g_watcher < 0) PyErr_Clear();  // none free: plan_new refuses, the Python path stays
     PyObject *m = PyModule_Create(&module);
     if (m) PyModule_AddIntConstant(m, "sizeof_smo_tensor", (long)sizeof(smo_tensor));
+    if (m) PyModule_AddIntConstant(m, "sizeof_smo_adamw_tensor", (long)sizeof(smo_adamw_tensor));
     return m;
 }

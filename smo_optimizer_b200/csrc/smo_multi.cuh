@@ -1,0 +1,91 @@
+// smo_multi.cuh -- many tensors in one launch, for the elementwise kernels.
+//
+// The descriptors travel as a kernel parameter (no copy to the device, nothing
+// to keep alive, and a captured graph holds its own).  Work is cut into chunks
+// of a fixed number of elements, numbered through all tensors of the launch.
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "smo_b200.h"
+#include "smo_common.cuh"
+#include "smo_internal.cuh"
+
+namespace smo {
+
+// 32,764 bytes is the most that one launch's parameters may hold
+constexpr size_t kMaxParamBytes = 32764;
+
+// index of the tensor that holds chunk `c`: the last i with start[i] <= c
+__device__ __forceinline__ int tensor_of(const int32_t *start, int n, int32_t c) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (start[mid] <= c) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// Eight consecutive elements as fp32, and back.  `p` must be 16-byte aligned.
+template <class T>
+__device__ __forceinline__ void ld8(const T *p, float (&x)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+        const uint4 a = *reinterpret_cast<const uint4 *>(p);
+        const T *e = reinterpret_cast<const T *>(&a);
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = ld<T>(e + k);
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void st8(T *p, const float (&x)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4 *>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        uint4 a;
+        T *e = reinterpret_cast<T *>(&a);
+#pragma unroll
+        for (int k = 0; k < 8; k++) st<T>(e + k, x[k]);
+        *reinterpret_cast<uint4 *>(p) = a;
+    }
+}
+
+// The first `left` (at most 8) of eight consecutive elements; 0 behind them.
+template <class T>
+__device__ __forceinline__ void ld8_part(const T *p, int64_t left, float (&x)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; k++) x[k] = k < left ? ld<T>(p + k) : 0.0f;
+}
+
+template <class T>
+__device__ __forceinline__ void st8_part(T *p, int64_t left, const float (&x)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+        if (k < left) st<T>(p + k, x[k]);
+}
+
+inline bool is_aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
+inline size_t dtype_bytes(int32_t dtype) { return dtype == SMO_DTYPE_F32 ? 4 : 2; }
+inline bool known_dtype(int32_t dtype) {
+    return dtype == SMO_DTYPE_F32 || dtype == SMO_DTYPE_BF16 || dtype == SMO_DTYPE_F16;
+}
+
+// smo_gradnorm.cu: the norm of n gradients (grad_of(items, i) is the i-th) into
+// norm_out (may be null), and the factor min(1, max_norm / (norm + 1e-6)), times
+// *scale where given, into *coef_out (a device float in the workspace; written
+// only with max_norm > 0).
+using GradOf = smo_grad (*)(const void *items, int32_t i);
+size_t grad_norm_workspace(int32_t n);
+int grad_norm_enqueue(GradOf grad_of, const void *items, int32_t n, const float *scale, float max_norm,
+                      float *norm_out, void *workspace, float **coef_out, cudaStream_t stream);
+
+}  // namespace smo

@@ -185,6 +185,8 @@ def _host_ext():
                 from e
         if _smo_host.sizeof_smo_tensor != _lib.TENSOR_DTYPE.itemsize:
             raise _lib.SmoError("_smo_host was built against another smo_tensor layout")
+        if _smo_host.sizeof_smo_adamw_tensor != _lib.ADAMW_DTYPE.itemsize:
+            raise _lib.SmoError("_smo_host was built against another smo_adamw_tensor layout")
         _HOST_EXT = _smo_host
     return _HOST_EXT
 

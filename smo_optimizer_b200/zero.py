@@ -32,6 +32,7 @@ import torch
 import torch.distributed as dist
 
 from . import _host
+from .adamw import AdamW8bit, _AdamWBase
 
 
 def step_bytes(shape, kind: str, k_ratio: float = 0.25, block: int = 64, compress_conv: bool = False,
@@ -59,6 +60,31 @@ def step_bytes(shape, kind: str, k_ratio: float = 0.25, block: int = 64, compres
         qb = _host.pooled_q_block(view[1], (h, w), block)
         return 3 * elem * n + 4 * c + 4 * elem * _host.num_blocks(c, qb)
     return 3 * elem * n + 4 * elem * c
+
+
+def adamw_step_bytes(shape, eight_bit: bool, block: int = 128, min_8bit_numel: int = 4096, elem: int = 4,
+                     master: bool = False) -> int:
+    """Algorithmic HBM bytes of one tensor's AdamW step, for parameters of ``elem`` bytes.
+
+    p r+w, g r (with a master copy of fp32: that r+w, p w, g r); moments r+w: 16 B/elem in fp32,
+    4 B/elem + 16 B/block in 8 bits.
+    """
+    n = 1
+    for s in shape:
+        n *= int(s)
+    moved = (2 * elem + 8 if master and elem < 4 else 3 * elem) * n
+    if eight_bit and n >= min_8bit_numel:
+        return moved + 4 * n + 16 * _host.num_blocks(n, block)
+    return moved + 16 * n
+
+
+def _step_cost(p, optimizer_cls, kwargs) -> int:
+    if issubclass(optimizer_cls, _AdamWBase):
+        return adamw_step_bytes(p.shape, issubclass(optimizer_cls, AdamW8bit), kwargs.get("block_size", 128),
+                                kwargs.get("min_8bit_numel", 4096), p.element_size(),
+                                kwargs.get("master_weights", False))
+    return step_bytes(p.shape, optimizer_cls.__name__, kwargs.get("k_ratio", kwargs.get("k") or 0.25),
+                      kwargs.get("block_size", 64), kwargs.get("compress_conv", False))
 
 
 def lpt_partition(costs, world: int):
@@ -159,7 +185,7 @@ class FlatParams:
 
 
 class Zero1:
-    """ZeRO-1 wrapper around ``SMO`` / ``SMO8bit``.
+    """ZeRO-1 wrapper around ``SMO`` / ``SMO8bit`` / ``AdamW`` / ``AdamW8bit``.
 
     ``Zero1(params, SMO8bit, lr=..., ...)`` builds the inner optimizer over the
     tensors this rank owns.  ``step()`` steps them and then exchanges the
@@ -178,9 +204,10 @@ class Zero1:
         self.world = dist.get_world_size(process_group) if dist.is_initialized() else 1
         self.rank = dist.get_rank(process_group) if dist.is_initialized() else 0
         self.params = [p for p in params]
-        kind = optimizer_cls.__name__
-        costs = [step_bytes(p.shape, kind, kwargs.get("k_ratio", kwargs.get("k") or 0.25),
-                            kwargs.get("block_size", 64), kwargs.get("compress_conv", False)) for p in self.params]
+        if self.world > 1 and kwargs.get("max_grad_norm") is not None:
+            raise ValueError("max_grad_norm: a rank's optimizer sees the gradients of its own tensors only; "
+                             "clip before Zero1.step()")
+        costs = [_step_cost(p, optimizer_cls, kwargs) for p in self.params]
         self.owner = lpt_partition(costs, self.world)
         self.costs = costs
         self.flat = None
