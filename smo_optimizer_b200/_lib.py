@@ -148,6 +148,12 @@ def step(table: np.ndarray, workspace_ptr: int, workspace_bytes: int, stream: in
     check(load().smo_step(table.ctypes.data, len(table), workspace_ptr, workspace_bytes, stream), "smo_step")
 
 
+_addresses = {}
+
+
 def address(name: str) -> int:
     """Address of a library function, for the host extension to call."""
-    return ctypes.cast(getattr(load(), name), ctypes.c_void_p).value
+    got = _addresses.get(name)
+    if got is None:
+        got = _addresses[name] = ctypes.cast(getattr(load(), name), ctypes.c_void_p).value
+    return got

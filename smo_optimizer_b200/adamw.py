@@ -20,7 +20,7 @@ from itertools import chain
 
 import numpy as np
 import torch
-from torch.optim.optimizer import Optimizer
+from torch.optim.optimizer import Optimizer, _global_optimizer_post_hooks, _global_optimizer_pre_hooks
 
 from . import _host, _lib
 from .optimizers import _DTYPE_CODES, _host_ext, _named, _same_dense_layout, protected_param_groups
@@ -42,11 +42,25 @@ def _stream(dev) -> int:
 # ---------------------------------------------------------------- gradient norms
 
 
-def _gradients(parameters, what):
-    if torch.is_tensor(parameters):
-        parameters = [parameters]
-    grads = [p.grad for p in parameters]
-    grads = [g for g in grads if g is not None]
+def _norm(parameters, max_norm, what):
+    lib = _lib.load()
+    ext, fn, ws = _host_ext(), _lib.address("smo_grad_norm"), _lib.address("smo_grad_norm_workspace_size")
+    parameters = [parameters] if torch.is_tensor(parameters) else list(parameters)
+    got = ext.grad_norm(parameters, max_norm, fn, ws)
+    if got is None:
+        got = _norm_of_copies(parameters, max_norm, what, ext, fn, ws)
+        if got is None:
+            return torch.zeros(())
+    if got[0]:
+        _lib.check(got[0], what)
+    return got[1]
+
+
+@torch.no_grad()
+def _norm_of_copies(parameters, max_norm, what, ext, fn, ws):
+    """Refusals, no gradients at all (None), and gradients with gaps or repeated
+    elements: those are taken as copies, written back when clipped."""
+    grads = [p.grad for p in parameters if p.grad is not None]
     for g in grads:
         if g.is_sparse:
             raise RuntimeError(f"{what} does not support sparse gradients.")
@@ -56,26 +70,21 @@ def _gradients(parameters, what):
             raise TypeError(f"{what} (B200 build) takes fp32, bf16 or fp16 gradients; got {g.dtype}")
         if g.device != grads[0].device:
             raise RuntimeError(f"{what} takes the gradients of one device; got {grads[0].device} and {g.device}")
-    return grads
+    if not grads:
+        return None
+    holders = []
+    for g in grads:
+        holder = torch.nn.Parameter(torch.empty_like(g, memory_format=torch.contiguous_format))
+        holder.grad = g.contiguous()
+        holders.append(holder)
+    got = ext.grad_norm(holders, max_norm, fn, ws)
+    if max_norm > 0:
+        for g, h in zip(grads, holders):
+            if h.grad.data_ptr() != g.data_ptr():
+                g.copy_(h.grad)
+    return got
 
 
-def _norm(grads, max_norm, what):
-    lib = _lib.load()
-    ext, fn, ws = _host_ext(), _lib.address("smo_grad_norm"), _lib.address("smo_grad_norm_workspace_size")
-    got = ext.grad_norm(grads, max_norm, fn, ws)
-    if got is None:
-        # gradients with gaps or repeated elements: on copies, written back when clipped
-        copies = [g.contiguous() for g in grads]
-        got = ext.grad_norm(copies, max_norm, fn, ws)
-        if max_norm > 0:
-            for g, c in zip(grads, copies):
-                if c is not g:
-                    g.copy_(c)
-    _lib.check(got[0], what)
-    return got[1]
-
-
-@torch.no_grad()
 def grad_norm(parameters) -> torch.Tensor:
     """The 2-norm over the gradients of all ``parameters`` (an iterable, or one
     parameter) as one vector: an fp32 tensor of no dimensions on their device.
@@ -83,14 +92,10 @@ def grad_norm(parameters) -> torch.Tensor:
     Parameters without a gradient are left out.  Each gradient is read once;
     squares and sums are held in double, in an order that depends on the sizes
     alone, so the same gradients always give the same bits.  Nothing
-    synchronises."""
-    grads = _gradients(parameters, "grad_norm")
-    if not grads:
-        return torch.zeros(())
-    return _norm(grads, 0.0, "grad_norm")
+    synchronises.  Without any gradient: 0, on the CPU."""
+    return _norm(parameters, 0.0, "grad_norm")
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     """Multiplies the gradients of all ``parameters`` in place by
     ``min(1, max_norm / (norm + 1e-6))`` and returns ``norm``, their 2-norm before
@@ -102,10 +107,7 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     max_norm = float(max_norm)
     if not max_norm > 0.0:
         raise ValueError(f"Invalid max_norm: {max_norm}")
-    grads = _gradients(parameters, "clip_grad_norm_")
-    if not grads:
-        return torch.zeros(())
-    return _norm(grads, max_norm, "clip_grad_norm_")
+    return _norm(parameters, max_norm, "clip_grad_norm_")
 
 
 # ---------------------------------------------------------------- optimizers
@@ -259,6 +261,16 @@ class _AdamWBase(Optimizer):
         ``grad_scale``: an fp32 tensor of one element on the parameters' device;
         the step multiplies every gradient by it (and leaves the gradients as
         they are).  ``max_grad_norm`` bounds the scaled gradients' norm."""
+        # torch's wrapper around step() costs 7.6 us, more than a small step's own
+        # host work: entered only for what it does, hooks and profiler records
+        if (self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or _global_optimizer_pre_hooks
+                or _global_optimizer_post_hooks or torch.autograd._profiler_enabled()):
+            return self._hooked_step(closure, grad_scale)
+        return self._step(closure, grad_scale)
+
+    step.hooked = True  # torch's Optimizer wraps a step() without this mark
+
+    def _step(self, closure, grad_scale):
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -281,6 +293,8 @@ class _AdamWBase(Optimizer):
                 self._plan = None
                 self._slow_step(items, grad_scale)
         return loss
+
+    _hooked_step = Optimizer.profile_hook_step(_step)
 
     def _scale_address(self, grad_scale, index):
         if grad_scale is None:

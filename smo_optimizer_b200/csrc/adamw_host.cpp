@@ -449,8 +449,8 @@ PyObject *adamw_moments(PyObject *, PyObject *args) {
     }
 }
 
-// grad_norm([gradient], max_norm, norm_fn_addr, workspace_fn_addr) -> (status, norm tensor), or None where a
-// gradient is not on the first one's CUDA device, of a known type and one span of memory
+// grad_norm([parameter], max_norm, norm_fn_addr, workspace_fn_addr) -> (status, norm tensor), or None where a
+// gradient is not on the first one's CUDA device, of a known type and one span of memory, or there is none
 PyObject *grad_norm(PyObject *, PyObject *args) {
     PyObject *list;
     float max_norm;
@@ -464,7 +464,8 @@ PyObject *grad_norm(PyObject *, PyObject *args) {
         for (Py_ssize_t i = 0; i < n; i++) {
             PyObject *o = PyList_GET_ITEM(list, i);
             if (!THPVariable_Check(o)) Py_RETURN_NONE;
-            const at::Tensor &g = THPVariable_Unpack(o);
+            const at::Tensor &g = THPVariable_Unpack(o).grad();
+            if (!g.defined()) continue;
             const int32_t dt = dtype_code(g.scalar_type());
             if (dt < 0 || !g.is_cuda() || g.layout() != c10::kStrided || !g.is_non_overlapping_and_dense())
                 Py_RETURN_NONE;
@@ -474,12 +475,12 @@ PyObject *grad_norm(PyObject *, PyObject *args) {
         }
         if (device < 0) Py_RETURN_NONE;
         c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
-        const size_t bytes = ((WorkspaceFn)(uintptr_t)ws_fn)((int32_t)n);
+        const size_t bytes = ((WorkspaceFn)(uintptr_t)ws_fn)((int32_t)table.size());
         const auto on = at::TensorOptions().device(c10::Device(c10::kCUDA, (c10::DeviceIndex)device));
         at::Tensor out = at::empty({}, on.dtype(c10::ScalarType::Float));
         at::Tensor ws = at::empty({(int64_t)bytes}, on.dtype(c10::ScalarType::Byte));
         cudaStream_t stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
-        const int rc = ((GradNormFn)(uintptr_t)fn)(table.data(), (int32_t)n, max_norm, (float *)out.data_ptr(),
+        const int rc = ((GradNormFn)(uintptr_t)fn)(table.data(), (int32_t)table.size(), max_norm, (float *)out.data_ptr(),
                                                    ws.data_ptr(), bytes, (void *)stream);
         return Py_BuildValue("iN", rc, THPVariable_Wrap(out));
     } catch (const std::exception &e) {

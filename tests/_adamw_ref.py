@@ -80,11 +80,20 @@ def decode(c, s, top):
 
 
 class Plain32:
-    """The definition in fp32; ``block``: 8-bit moments (None: fp32)."""
+    """The definition in fp32; ``block``: 8-bit moments (None: fp32).
+
+    ``tol_p`` bounds how far the parameter of the 8-bit step may be off, whose
+    quotient is not rounded as defined: the reciprocal is within 2 half steps
+    and its product rounds once more where the quotient rounds once; the
+    denominator's and the parameter's multiply-adds round once instead of
+    twice (1 for the denominator, 2 for the parameter).  With the difference
+    of each pair counted for both: 8 half steps of the update, 4 of the
+    parameter.  A stored type then rounds either way: one of its steps."""
 
     def __init__(self, p, block=None, round_to=None):
         self.p = p.astype(np.float32).reshape(-1)
         self.block, self.round_to, self.t = block, round_to, 0
+        self.tol_p = np.zeros(self.p.size)
         self.m = np.zeros_like(self.p)
         self.v = np.zeros_like(self.p)
         if block:
@@ -108,8 +117,13 @@ class Plain32:
             self.v = self.v * s["b2"] + (g * s["o2"]) * g
             root = np.sqrt(self.v)
             upd = (self.m * s["size"]) / (root * s["rs"] + s["eps"])
+            self.tol_p = self.tol_p + 8 * EPS32 * np.abs(upd.astype(np.float64)) + 4 * EPS32 * np.abs(self.p)
             self.p = self.p * s["decay"] - upd
-        if self.round_to is not None:
-            self.p = self.round_to(self.p)
+            if self.round_to is not None:
+                self.p = self.round_to(self.p)
+                # the types' steps: from eps of the value, and not below their smallest number's
+                eps = 2.0 ** -7 if self.round_to(np.float32([1 + 2.0 ** -9]))[0] == 1 else 2.0 ** -10
+                least = eps * (2.0 ** -126 if eps == 2.0 ** -7 else 2.0 ** -14)
+                self.tol_p = self.tol_p + np.maximum(eps * np.abs(self.p), least)
         if self.block:
             self.codes = [encode(self.m, 127, self.block), encode(root, 255, self.block)]

@@ -156,3 +156,28 @@ def test_zero_cost_model():
     assert adamw_step_bytes((10, 10), True) == 28 * 100
     assert adamw_step_bytes((100, 100), False, elem=2, master=True) == 28 * 10000
     assert adamw_step_bytes((100, 100), False, elem=2) == 22 * 10000
+
+
+@pytest.mark.parametrize("cls", [AdamW, AdamW8bit])
+def test_step_hooks_and_schedulers(cls):
+    """Hooks of one optimizer and of all, profiler records and a scheduler see every step."""
+    p = _p()
+    opt = cls([p], lr=0.5)
+    seen = []
+    handles = [opt.register_step_pre_hook(lambda o, args, kw: seen.append("pre")),
+               opt.register_step_post_hook(lambda o, args, kw: seen.append("post")),
+               torch.optim.optimizer.register_optimizer_step_post_hook(lambda o, args, kw: seen.append("all"))]
+    opt.step()
+    assert seen == ["pre", "post", "all"] or sorted(seen) == ["all", "post", "pre"]
+    for h in handles:
+        h.remove()
+    opt.step()
+    assert len(seen) == 3
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        opt.step()
+    assert any(f"Optimizer.step#{cls.__name__}.step" in e.key for e in prof.key_averages())
+    assert opt.step(lambda: 3.0) == 3.0
+    sched = torch.optim.lr_scheduler.StepLR(opt, 1, gamma=0.5)
+    opt.step()
+    sched.step()
+    assert opt.param_groups[0]["lr"] == 0.25

@@ -62,6 +62,15 @@ def _same(a, b, what):
     assert ok.all(), f"{what}: {np.flatnonzero(~ok.reshape(-1))[:8]} of {ok.size}"
 
 
+def _check_param(got, ref, what):
+    """The parameter's bits with fp32 moments; within tol_p with 8-bit moments."""
+    if not ref.block:
+        return _same(got, ref.p, what)
+    with np.errstate(invalid="ignore"):
+        ok = (got == ref.p) | (np.isnan(got) & np.isnan(ref.p)) | (np.abs(got.astype(np.float64) - ref.p) <= ref.tol_p)
+    assert ok.all(), f"{what}: {np.flatnonzero(~ok)[:8]} of {ok.size}"
+
+
 def _check_codes(state, ref, what):
     for k, (c, s) in zip("mv", ref.codes):
         _same(state[k + "_q"].cpu().numpy().astype(np.int32), c, f"{what}: {k}_q")
@@ -151,7 +160,7 @@ def test_step_gives_the_definitions_bits(dtype, block, clip):
         if clip:
             assert float(opt.last_grad_norm) == total
     for p, r, n in zip(params, refs, SIZES):
-        _same(_np(p), r.p, n)
+        _check_param(_np(p), r, n)
         if block is None:
             _same(_np(opt.state[p]["exp_avg"]), r.m, n)
             _same(_np(opt.state[p]["exp_avg_sq"]), r.v, n)
@@ -191,7 +200,7 @@ def test_odd_values(kind, block):
         p.grad = torch.from_numpy(g).cuda()
         opt.step()
         ref.step(g, *ARGS)
-        _same(_np(p), ref.p, (kind, step))
+        _check_param(_np(p), ref, (kind, step))
         if block:
             _check_codes(opt.state[p], ref, (kind, step))
         else:
@@ -228,7 +237,7 @@ def test_unaligned_views_touch_only_their_elements(lead, dtype, block):
             r.step(_np(p.grad), *ARGS)
     assert torch.equal(flat[:lead], before)
     for p, r in zip(params, refs):
-        _same(_np(p), r.p, (lead, p.numel()))
+        _check_param(_np(p), r, (lead, p.numel()))
         if block:
             _check_codes(opt.state[p], r, (lead, p.numel()))
 
@@ -290,7 +299,7 @@ def test_many_tensors_types_groups_and_missing_gradients(block):
         if steps[i]:
             assert opt.state[p]["step"] == steps[i]
             assert ("m_q" in opt.state[p]) == bool(ref.block)
-        _same(_np(p), ref.p, (i, p.numel()))
+        _check_param(_np(p), ref, (i, p.numel()))
 
 
 @pytest.mark.parametrize("block", [None, 256])
@@ -346,7 +355,7 @@ def test_plan_follows_replaced_tensors():
     refs.append(Plain32(_np(extra[0])))
     both(3e-3)
     for p, r in zip(params, refs):
-        _same(_np(p), r.p, p.numel())
+        _check_param(_np(p), r, p.numel())
 
 
 # ---------------------------------------------------------------- scaling
@@ -364,7 +373,7 @@ def test_grad_scale_and_clipping_together():
     c = np.float32(0.25) / (total + np.float32(1e-6)) * np.float32(0.125)
     for p, r in zip(params, refs):
         r.step(_np(p.grad), *ARGS, scale=c)
-        _same(_np(p), r.p, p.numel())
+        _check_param(_np(p), r, p.numel())
     with pytest.raises(TypeError):
         opt.step(grad_scale=0.5)
     with pytest.raises(TypeError):
@@ -536,7 +545,7 @@ def test_runs_on_the_current_stream():
             ref.step(2 * g, *ARGS)
         assert float(grad_norm(params)) == pytest.approx(float(np.linalg.norm(2.0 * g.astype(np.float64))), rel=1e-6)
     side.synchronize()
-    _same(_np(params[0]), ref.p, "side stream")
+    _check_param(_np(params[0]), ref, "side stream")
 
 
 def test_more_than_2_to_31_elements():
@@ -552,7 +561,7 @@ def test_more_than_2_to_31_elements():
     g[-5000:] = _np(tail)
     ref = Plain32(np.zeros(n - first), 128, _rounder(torch.bfloat16))
     ref.step(g, *ARGS)
-    _same(_np(p[first:]), ref.p, "tail")
+    _check_param(_np(p[first:]), ref, "tail")
     for k, (c, s) in zip("mv", ref.codes):
         _same(opt.state[p][k + "_q"][first // 128:].cpu().numpy().astype(np.int32), c, k)
         _same(opt.state[p][k + "_s"][first // 128:].cpu().numpy(), s, k)
