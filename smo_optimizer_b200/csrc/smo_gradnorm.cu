@@ -15,40 +15,51 @@ namespace smo {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunk = kThreads * 8 * 4;  // elements of a chunk
+constexpr int kVecs = 4;                  // eight-element accesses of a thread and chunk
+constexpr int kChunk = kThreads * 8 * kVecs;
 constexpr int kCap = 1024;                // tensors of one launch
-constexpr int kParts = 148 * 8;           // CTAs of one launch at most: one partial sum each
+constexpr int kFewCap = 128;              // where there are fewer, a smaller parameter: 2 us less to launch
+// CTAs of one launch at most, one partial sum each: four times what is resident,
+// so that sets of up to 39M elements have one chunk a CTA and the last CTAs level
+// out.  38M bf16 elements in 148 tensors, read from L2: 22.6 us with as many CTAs
+// as are resident, 16.4 us so; 757M: 227 and 220 us.  Chunks of half the size:
+// 26.6 and 232 us.
+constexpr int kParts = 148 * 8 * 4;
+constexpr int kSumThreads = 1024;         // of the CTA that adds the partial sums
 
 struct GradDesc {
     void *g;
     int64_t n;
 };
 
+template <int CAP>
 struct GradBatch {
     int32_t n;
     double *part;
     const float *coef;
-    int32_t start[kCap + 1];
-    GradDesc d[kCap];
+    int32_t start[CAP + 1];
+    GradDesc d[CAP];
 };
-static_assert(sizeof(GradBatch) <= kMaxParamBytes, "launch parameters");
+static_assert(sizeof(GradBatch<kCap>) <= kMaxParamBytes, "launch parameters");
 
 // sum over the CTA, in thread 0
+template <int THREADS>
 __device__ __forceinline__ double cta_sum(double x) {
-    __shared__ double warp[kThreads / 32];
+    __shared__ double warp[THREADS / 32];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) x += __shfl_down_sync(0xffffffffu, x, o);
     if ((threadIdx.x & 31) == 0) warp[threadIdx.x >> 5] = x;
     __syncthreads();
-    x = threadIdx.x < kThreads / 32 ? warp[threadIdx.x] : 0.0;
+    x = threadIdx.x < THREADS / 32 ? warp[threadIdx.x] : 0.0;
     if (threadIdx.x < 32)
 #pragma unroll
-        for (int o = kThreads / 64; o > 0; o >>= 1) x += __shfl_down_sync(0xffffffffu, x, o);
+        for (int o = THREADS / 64; o > 0; o >>= 1) x += __shfl_down_sync(0xffffffffu, x, o);
     return x;
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__ GradBatch b) {
+template <class T, int CAP>
+__global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__ GradBatch<CAP> b) {
+    let_next_start();
     const int32_t total = b.start[b.n];
     double acc = 0.0;
     int t = tensor_of(b.start, b.n, blockIdx.x);
@@ -60,7 +71,7 @@ __global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__
         const int64_t end = base + kChunk < d.n ? base + kChunk : d.n;
         if (((uintptr_t)g & 15) == 0 && base + kChunk <= d.n) {
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
+            for (int u = 0; u < kVecs; u++) {
                 float x[8];
                 ld8<T>(g + base + (u * kThreads + threadIdx.x) * 8, x);
 #pragma unroll
@@ -73,45 +84,58 @@ __global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__
             }
         }
     }
-    acc = cta_sum(acc);
+    acc = cta_sum<kThreads>(acc);
     if (threadIdx.x == 0) b.part[blockIdx.x] = acc;
 }
 
+struct NormArgs {
+    const double *part;
+    int32_t n;
+    const float *scale;
+    float max_norm;
+    float *norm_out, *coef;
+};
+
 // norm = sqrt(sum of the parts) * |scale|; coef = min(1, max_norm / (norm + 1e-6)) * scale
-__global__ void __launch_bounds__(kThreads) norm_kernel(const double *part, int32_t n, const float *scale,
-                                                        float max_norm, float *norm_out, float *coef) {
+__global__ void __launch_bounds__(kSumThreads) norm_kernel(NormArgs a) {
+    let_next_start();
+    wait_for_previous();
     double acc = 0.0;
-    for (int32_t i = threadIdx.x; i < n; i += kThreads) acc += part[i];
-    acc = cta_sum(acc);
+    for (int32_t i = threadIdx.x; i < a.n; i += kSumThreads) acc += a.part[i];
+    acc = cta_sum<kSumThreads>(acc);
     if (threadIdx.x != 0) return;
-    const float s = scale ? *scale : 1.0f;
+    const float s = a.scale ? *a.scale : 1.0f;
     const float norm = (float)(sqrt(acc) * (double)fabsf(s));
-    if (norm_out) *norm_out = norm;
-    if (max_norm > 0.0f) {
-        const float c = __fdiv_rn(max_norm, __fadd_rn(norm, 1e-6f));
-        *coef = __fmul_rn(c > 1.0f ? 1.0f : c, s);  // a NaN norm gives a NaN factor
+    if (a.norm_out) *a.norm_out = norm;
+    if (a.max_norm > 0.0f) {
+        const float c = __fdiv_rn(a.max_norm, __fadd_rn(norm, 1e-6f));
+        *a.coef = __fmul_rn(c > 1.0f ? 1.0f : c, s);  // a NaN norm gives a NaN factor
     }
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ GradBatch b) {
-    const int t = tensor_of(b.start, b.n, blockIdx.x);
+template <class T, int CAP>
+__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ GradBatch<CAP> b) {
+    // from the last chunk to the first: what the norm read last is still in L2
+    const int32_t chunk = (int32_t)(gridDim.x - 1 - blockIdx.x), t = tensor_of(b.start, b.n, chunk);
     const GradDesc &d = b.d[t];
-    const float c = *b.coef;
     T *g = (T *)d.g;
-    const int64_t base = (int64_t)(blockIdx.x - b.start[t]) * kChunk;
+    const int64_t base = (int64_t)(chunk - b.start[t]) * kChunk;
     const int64_t end = base + kChunk < d.n ? base + kChunk : d.n;
     if (((uintptr_t)g & 15) == 0 && base + kChunk <= d.n) {
-        float x[4][8];
+        float x[kVecs][8];
 #pragma unroll
-        for (int u = 0; u < 4; u++) ld8<T>(g + base + (u * kThreads + threadIdx.x) * 8, x[u]);
+        for (int u = 0; u < kVecs; u++) ld8<T>(g + base + (u * kThreads + threadIdx.x) * 8, x[u]);
+        wait_for_previous();
+        const float c = *b.coef;
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
+        for (int u = 0; u < kVecs; u++) {
 #pragma unroll
             for (int k = 0; k < 8; k++) x[u][k] = __fmul_rn(x[u][k], c);
             st8<T>(g + base + (u * kThreads + threadIdx.x) * 8, x[u]);
         }
     } else {
+        wait_for_previous();
+        const float c = *b.coef;
         for (int64_t i = base + threadIdx.x; i < end; i += kThreads) st<T>(g + i, __fmul_rn(ld<T>(g + i), c));
     }
 }
@@ -127,53 +151,59 @@ int cuda_status(cudaError_t e) {
 // launches over n tensors: full batches, and up to one more for each dtype
 int32_t most_launches(int32_t n) { return n / kCap + 3; }
 
-template <class T>
-int launch(const GradBatch &b, bool scale, int32_t &parts, cudaStream_t s) {
-    if (b.n == 0) return SMO_OK;
+template <class T, int CAP>
+int launch(const GradBatch<CAP> &b, int32_t &parts, cudaStream_t s) {
     const int32_t chunks = b.start[b.n];
-    if (scale) {
-        scale_kernel<T><<<(unsigned)chunks, kThreads, 0, s>>>(b);
+    cudaError_t e;
+    if (b.coef) {
+        e = launch_batch(scale_kernel<T, CAP>, (unsigned)chunks, kThreads, b, true, s);
     } else {
         const int32_t ctas = chunks < kParts ? chunks : kParts;
-        sumsq_kernel<T><<<(unsigned)ctas, kThreads, 0, s>>>(b);
+        e = launch_batch(sumsq_kernel<T, CAP>, (unsigned)ctas, kThreads, b, false, s);
         parts += ctas;
     }
     g_launches++;
-    return cuda_status(cudaGetLastError());
+    return cuda_status(e);
 }
 
-int launch(const GradBatch &b, int32_t dtype, bool scale, int32_t &parts, cudaStream_t s) {
-    if (dtype == SMO_DTYPE_F32) return launch<float>(b, scale, parts, s);
-    if (dtype == SMO_DTYPE_BF16) return launch<__nv_bfloat16>(b, scale, parts, s);
-    return launch<__half>(b, scale, parts, s);
-}
-
-// every gradient, batched by dtype: partial sums (coef null) or scaling by *coef
-int run(GradOf grad_of, const void *items, int32_t n, double *part, const float *coef, int32_t &parts,
-        cudaStream_t s) {
-    static thread_local GradBatch b;
-    for (int32_t dt = SMO_DTYPE_F32; dt <= SMO_DTYPE_F16; dt++) {
-        b.n = 0;
-        b.start[0] = 0;
-        b.coef = coef;
-        for (int32_t i = 0; i <= n; i++) {
-            const bool end = i == n;
-            const smo_grad g = end ? smo_grad{} : grad_of(items, i);
-            if (!end && (g.dtype != dt || g.n == 0)) continue;
-            const int64_t chunks = (g.n + kChunk - 1) / kChunk;
-            if (end || b.n == kCap) {
-                b.part = part + parts;
-                const int st = launch(b, dt, coef != nullptr, parts, s);
-                if (st != SMO_OK) return st;
-                b.n = 0;
-                if (end) break;
-            }
-            b.d[b.n] = GradDesc{g.grad, g.n};
-            b.start[b.n + 1] = b.start[b.n] + (int32_t)chunks;
-            b.n++;
+// the gradients of one dtype: partial sums (coef null) or scaling by *coef
+template <class T, int CAP>
+int run_type(GradOf grad_of, const void *items, int32_t n, int32_t dtype, double *part, const float *coef,
+             int32_t &parts, cudaStream_t s) {
+    static thread_local GradBatch<CAP> b;
+    b.n = 0;
+    b.start[0] = 0;
+    b.coef = coef;
+    for (int32_t i = 0; i <= n; i++) {
+        const bool end = i == n;
+        const smo_grad g = end ? smo_grad{} : grad_of(items, i);
+        if (!end && (g.dtype != dtype || g.n == 0)) continue;
+        if (b.n > 0 && (end || b.n == CAP)) {
+            b.part = part + parts;
+            const int st = launch<T, CAP>(b, parts, s);
+            if (st != SMO_OK) return st;
+            b.n = 0;
         }
+        if (end) break;
+        b.d[b.n] = GradDesc{g.grad, g.n};
+        b.start[b.n + 1] = b.start[b.n] + (int32_t)((g.n + kChunk - 1) / kChunk);
+        b.n++;
     }
     return SMO_OK;
+}
+
+// every gradient, batched by dtype
+int run(GradOf grad_of, const void *items, int32_t n, double *part, const float *coef, int32_t &parts,
+        cudaStream_t s) {
+    int st = SMO_OK;
+    const bool few = n <= kFewCap;
+    for (int32_t dt = SMO_DTYPE_F32; dt <= SMO_DTYPE_F16 && st == SMO_OK; dt++) {
+        const auto f = dt == SMO_DTYPE_F32    ? (few ? run_type<float, kFewCap> : run_type<float, kCap>)
+                       : dt == SMO_DTYPE_BF16 ? (few ? run_type<__nv_bfloat16, kFewCap> : run_type<__nv_bfloat16, kCap>)
+                                              : (few ? run_type<__half, kFewCap> : run_type<__half, kCap>);
+        st = f(grad_of, items, n, dt, part, coef, parts, s);
+    }
+    return st;
 }
 
 }  // namespace
@@ -204,10 +234,13 @@ int grad_norm_enqueue(GradOf grad_of, const void *items, int32_t n, const float 
     int32_t parts = 0;
     const int st = run(grad_of, items, n, part, nullptr, parts, s);
     if (st != SMO_OK) return st;
-    norm_kernel<<<1, kThreads, 0, s>>>(part, parts, scale, max_norm, norm_out, coef);
+    // it may start early only behind a partial sum, which itself started after
+    // everything before it had ended
+    const cudaError_t e = launch_batch(norm_kernel, 1, kSumThreads, NormArgs{part, parts, scale, max_norm, norm_out, coef},
+                                       parts > 0, s);
     g_launches++;
     if (coef_out) *coef_out = coef;
-    return cuda_status(cudaGetLastError());
+    return cuda_status(e);
 }
 
 }  // namespace smo

@@ -20,6 +20,29 @@ namespace smo {
 // 32,764 bytes is the most that one launch's parameters may hold
 constexpr size_t kMaxParamBytes = 32764;
 
+// Launch of a kernel whose one parameter is the batch.  `after`: it may start
+// while the kernel before it in the stream ends (programmatic dependent
+// launch); it then calls wait_for_previous() before it reads that kernel's results
+// or writes what that kernel reads.
+template <class B>
+cudaError_t launch_batch(void (*kernel)(B), unsigned ctas, unsigned threads, const B &b, bool after, cudaStream_t s) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = after ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, b);
+}
+
+// every kernel before this one in the stream has ended and its writes are visible
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// the next kernel may start as soon as every CTA has come here (or ended)
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // index of the tensor that holds chunk `c`: the last i with start[i] <= c
 __device__ __forceinline__ int tensor_of(const int32_t *start, int n, int32_t c) {
     int lo = 0, hi = n - 1;
