@@ -274,6 +274,18 @@ SMO_API size_t smo_grad_norm_workspace_size(int32_t n);
 SMO_API int smo_adamw_step(const smo_adamw_tensor *tensors, int32_t n, const float *grad_scale, float max_norm,
                            float *norm_out, void *workspace, size_t workspace_bytes, void *stream);
 
+/* A tensor's step count and hyperparameters where the scalars are formed on
+ * the device, so that a captured graph advances them with every replay. */
+typedef struct smo_adamw_schedule {
+    float *step;             /* device: steps taken so far */
+    const float *lr_dev;     /* device: the learning rate; NULL: lr */
+    double lr, beta1, beta2, eps, weight_decay;
+} smo_adamw_schedule;
+
+/* Adds 1 to each item's step and writes its scalars to out[i] (device memory,
+ * n of them), for smo_adamw_tensor.hp_dev.  Formed in double, rounded once. */
+SMO_API int smo_adamw_advance(const smo_adamw_schedule *items, int32_t n, smo_adamw_hyper *out, void *stream);
+
 /* The moments of SMO_ADAMW_8BIT tensors as 32-bit numbers: exp_avg = m and
  * exp_avg_sq = u * u receive what the codes stand for (only exp_avg,
  * exp_avg_sq, the codes, scales, n and q_block are read). */

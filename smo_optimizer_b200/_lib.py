@@ -62,6 +62,9 @@ ADAMW_DTYPE = np.dtype([
     ("hp", ADAMW_HYPER_DTYPE),
 ])
 
+SCHEDULE_DTYPE = np.dtype([("step", np.uint64), ("lr_dev", np.uint64)] +
+                          [(name, np.float64) for name in ("lr", "beta1", "beta2", "eps", "weight_decay")])
+
 GRAD_DTYPE = np.dtype([("grad", np.uint64), ("n", np.int64), ("dtype", np.int32), ("reserved", np.int32)])
 
 
@@ -107,6 +110,7 @@ def load():
         "smo_set_wait_limit": (i64, [i64]),
         "smo_inject_wait_timeout": (ctypes.c_int, [ctypes.c_int]),
         "smo_adamw_step": (ctypes.c_int, [P, i32, P, ctypes.c_float, P, P, sz, P]),
+        "smo_adamw_advance": (ctypes.c_int, [P, i32, P, P]),
         "smo_adamw_decode": (ctypes.c_int, [P, i32, P]),
         "smo_adamw_encode": (ctypes.c_int, [P, i32, P]),
         "smo_adamw_tensor_struct_size": (sz, []),

@@ -116,8 +116,10 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
 class _AdamWBase(Optimizer):
     _name = "AdamW"
 
-    def __init__(self, params, lr, betas, eps, weight_decay, master_weights, max_grad_norm, extra):
-        if not 0.0 <= lr:
+    def __init__(self, params, lr, betas, eps, weight_decay, master_weights, max_grad_norm, capturable, extra):
+        if torch.is_tensor(lr) and not capturable:
+            raise ValueError("lr as a tensor needs capturable=True")
+        if not torch.is_tensor(lr) and not 0.0 <= lr:
             raise ValueError(f"Invalid learning rate: {lr}")
         if not 0.0 <= eps:
             raise ValueError(f"Invalid epsilon value: {eps}")
@@ -131,17 +133,20 @@ class _AdamWBase(Optimizer):
             raise ValueError(f"Invalid max_grad_norm: {max_grad_norm}")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, **extra))
         self.master_weights = bool(master_weights)
+        self.capturable = bool(capturable)
         self.max_grad_norm = max_grad_norm
         # norm of the gradients that the last step saw, before clipping; kept
         # only with max_grad_norm, and overwritten by the next step
         self.last_grad_norm = None
         self._plan = None       # (capsule of the C++ host path, device index, number of tensors)
         self._workspace = {}    # device index -> (workspace, norm)
+        self._scalars = {}      # device index -> scalars of each tensor (capturable)
+        self._kept = []         # outgrown ones of the two, which captured graphs may hold
 
     # ---------------------------------------------------------------- state
 
     # torch's Optimizer pickles (and deep-copies) its groups and state only
-    _SETTINGS = ("master_weights", "max_grad_norm")
+    _SETTINGS = ("master_weights", "max_grad_norm", "capturable")
 
     def __getstate__(self):
         return dict(super().__getstate__(), **{k: getattr(self, k) for k in self._SETTINGS})
@@ -149,7 +154,8 @@ class _AdamWBase(Optimizer):
     def __setstate__(self, state):
         super().__setstate__(state)
         self._plan = None
-        self._workspace = {}
+        self._workspace, self._scalars = {}, {}
+        self._kept = getattr(self, "_kept", [])
         self.last_grad_norm = None
 
     def _eight_bit(self, p, group) -> bool:
@@ -157,7 +163,7 @@ class _AdamWBase(Optimizer):
 
     def _init_state(self, p, group):
         state = self.state[p]
-        state["step"] = 0
+        state["step"] = torch.zeros((), device=p.device) if self.capturable else 0
         if self._eight_bit(p, group):
             block = group["block_size"]
             nb = _host.num_blocks(p.numel(), block)
@@ -186,11 +192,25 @@ class _AdamWBase(Optimizer):
                                     f"gradients of the same dtype; got {p.dtype} / {grad.dtype}")
                 state = self.state[p]
                 if "step" not in state:
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError(f"{self._name}: the first step of a parameter cannot be captured (replays "
+                                           "would make its state anew); take one before the capture")
                     self._init_state(p, group)
+                state["step"] = self._step_value(p, state["step"])
                 if self.master_weights and p.dtype != torch.float32 and "master" not in state:
                     state["master"] = p.detach().to(torch.float32, memory_format=torch.preserve_format)
                 found.append((p, grad, state, group))
         return found
+
+    def _step_value(self, p, step):
+        """A step count as this optimizer keeps it."""
+        if not self.capturable:
+            return step if type(step) is int else int(step)
+        if torch.is_tensor(step):
+            if step.dtype == torch.float32 and step.device == p.device and step.numel() == 1:
+                return step
+            return step.to(dtype=torch.float32, device=p.device).reshape(())
+        return torch.full((), float(step), device=p.device)
 
     def load_state_dict(self, state_dict):
         """Loads what ``state_dict()`` of this class, of the other one here or of
@@ -214,7 +234,7 @@ class _AdamWBase(Optimizer):
             if not saved:
                 continue
             # torch's loader has cast every tensor to the parameter's type: take the saved ones
-            state = {"step": int(saved.get("step", 0))}
+            state = {"step": self._step_value(p, saved.get("step", 0))}
             for key, dtype in _STATE_DTYPES.items():
                 if torch.is_tensor(saved.get(key)):
                     state[key] = saved[key].to(device=p.device, dtype=dtype)
@@ -288,7 +308,8 @@ class _AdamWBase(Optimizer):
             if not items:
                 self.last_grad_norm = None
                 return loss
-            self._plan = _host_ext().adamw_plan(self.param_groups, self.state, _lib.address("smo_adamw_step"))
+            self._plan = _host_ext().adamw_plan(self.param_groups, self.state, _lib.address("smo_adamw_step"),
+                                                _lib.address("smo_adamw_advance") if self.capturable else 0)
             if self._plan is None or self._run_plan(grad_scale) < 0:
                 self._plan = None
                 self._slow_step(items, grad_scale)
@@ -311,16 +332,30 @@ class _AdamWBase(Optimizer):
         need = _lib.load().smo_grad_norm_workspace_size(tensors)
         kept = self._workspace.get(index)
         if kept is None or kept[0].numel() < need:
+            if kept is not None:
+                self._kept.append(kept)
             dev = torch.device("cuda", index)
             kept = (torch.empty(need, dtype=torch.uint8, device=dev), torch.zeros((), device=dev))
             self._workspace[index] = kept
         self.last_grad_norm = kept[1]
         return float(self.max_grad_norm), kept[1].data_ptr(), kept[0].data_ptr(), kept[0].numel()
 
+    def _scalar_address(self, index, tensors):
+        """Device memory for the scalars of so many tensors (capturable), or 0."""
+        if not self.capturable:
+            return 0
+        kept = self._scalars.get(index)
+        if kept is None or kept.shape[0] < tensors:
+            if kept is not None:
+                self._kept.append(kept)
+            kept = torch.empty((tensors, len(_lib.ADAMW_HYPER_DTYPE)), device=torch.device("cuda", index))
+            self._scalars[index] = kept
+        return kept.data_ptr()
+
     def _run_plan(self, grad_scale) -> int:
         cap, index, tensors = self._plan
         scale = self._scale_address(grad_scale, index)
-        rc = _host_ext().adamw_run(cap, scale, *self._norm_buffers(index, tensors))
+        rc = _host_ext().adamw_run(cap, self._scalar_address(index, tensors), scale, *self._norm_buffers(index, tensors))
         if rc > 0:
             self._check(rc)
         return rc
@@ -328,7 +363,7 @@ class _AdamWBase(Optimizer):
     def _check(self, rc):
         if rc == _lib.SMO_ERR_CAPTURE:
             raise RuntimeError(f"{self._name}.step cannot be captured into a CUDA graph: the step count and the learning "
-                               "rate are host values, which every replay would repeat")
+                               "rate are host values, which every replay would repeat (see capturable=True)")
         _lib.check(rc, "smo_adamw_step")
 
     def _slow_step(self, items, grad_scale):
@@ -348,15 +383,35 @@ class _AdamWBase(Optimizer):
             with torch.cuda.device(dev):
                 scale = self._scale_address(grad_scale, dev.index)
                 max_norm, norm, ws, nbytes = self._norm_buffers(dev.index, len(items))
+                if self.capturable:
+                    self._advance(dev, items, table)
                 self._check(_lib.load().smo_adamw_step(table.ctypes.data, len(table), scale, max_norm, norm, ws, nbytes,
                                                        _stream(dev)))
                 for dst, src in back:
                     dst.copy_(src)
-            for p, grad, state, group in items:
-                state["step"] += 1
+            if not self.capturable:
+                for p, grad, state, group in items:
+                    state["step"] += 1
 
-    @staticmethod
-    def _fill(rec, p, grad, state, group, back, keep):
+    def _advance(self, dev, items, table):
+        """Step counts and scalars of a slow step on the device."""
+        schedule = np.zeros(len(items), dtype=_lib.SCHEDULE_DTYPE)
+        out = self._scalar_address(dev.index, len(items))
+        for i, (rec, (p, grad, state, group)) in enumerate(zip(schedule, items)):
+            lr = group["lr"]
+            if torch.is_tensor(lr):
+                if lr.dtype != torch.float32 or lr.device != dev or lr.numel() != 1:
+                    raise TypeError(f"lr must be a number or an fp32 tensor of one element on {dev}")
+                rec["lr_dev"] = lr.data_ptr()
+            else:
+                rec["lr"] = lr
+            rec["step"] = state["step"].data_ptr()
+            rec["beta1"], rec["beta2"] = group["betas"]
+            rec["eps"], rec["weight_decay"] = group["eps"], group["weight_decay"]
+            table[i]["hp_dev"] = out + i * _lib.ADAMW_HYPER_DTYPE.itemsize
+        self._check(_lib.load().smo_adamw_advance(schedule.ctypes.data, len(schedule), out, _stream(dev)))
+
+    def _fill(self, rec, p, grad, state, group, back, keep):
         coded = all(k in state for k in _CODE_KEYS)
         floats = ("master",) if "master" in state else ()
         floats += () if coded else _FLOAT_KEYS
@@ -401,8 +456,9 @@ class _AdamWBase(Optimizer):
             rec["kind"], rec["q_block"] = _lib.SMO_ADAMW_8BIT, block
         else:
             rec["kind"] = _lib.SMO_ADAMW_F32
-        rec["hp"] = _host.adamw_scalars(group["lr"], group["betas"], group["eps"], group["weight_decay"],
-                                        state["step"] + 1)
+        if not self.capturable:
+            rec["hp"] = _host.adamw_scalars(group["lr"], group["betas"], group["eps"], group["weight_decay"],
+                                            state["step"] + 1)
 
 
 class AdamW(_AdamWBase):
@@ -416,14 +472,18 @@ class AdamW(_AdamWBase):
     ``min(1, max_grad_norm / (norm + 1e-6))`` within the step;
     ``last_grad_norm`` is then the norm (a device tensor, overwritten by the next
     step).
+    ``capturable``: the step can be captured into a CUDA graph and replayed.  The
+    step counts are then fp32 device tensors and the scalars are formed on the
+    device (one more launch); ``lr`` may be an fp32 device tensor, which replays
+    read.  Take a step before the capture: it makes the state.
 
     ``state[p]``: ``step`` (int), ``exp_avg``, ``exp_avg_sq``, with master weights
     ``master``."""
     _name = "AdamW"
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, master_weights=False,
-                 max_grad_norm=None):
-        super().__init__(params, lr, betas, eps, weight_decay, master_weights, max_grad_norm, {})
+                 max_grad_norm=None, capturable=False):
+        super().__init__(params, lr, betas, eps, weight_decay, master_weights, max_grad_norm, capturable, {})
 
 
 class AdamW8bit(_AdamWBase):
@@ -448,7 +508,8 @@ class AdamW8bit(_AdamWBase):
     _SETTINGS = _AdamWBase._SETTINGS + ("min_8bit_numel",)
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, block_size=128,
-                 min_8bit_numel=4096, master_weights=False, max_grad_norm=None, protect_output=False):
+                 min_8bit_numel=4096, master_weights=False, max_grad_norm=None, protect_output=False,
+                 capturable=False):
         if block_size not in BLOCK_SIZES:
             raise ValueError(f"Invalid block_size: {block_size}. Must be one of {BLOCK_SIZES}")
         if not 0 <= min_8bit_numel:
@@ -456,7 +517,7 @@ class AdamW8bit(_AdamWBase):
         if protect_output:
             params = protected_param_groups(_named(params), protect_output)
         self.min_8bit_numel = int(min_8bit_numel)
-        super().__init__(params, lr, betas, eps, weight_decay, master_weights, max_grad_norm,
+        super().__init__(params, lr, betas, eps, weight_decay, master_weights, max_grad_norm, capturable,
                          dict(block_size=block_size))
 
     def _eight_bit(self, p, group) -> bool:

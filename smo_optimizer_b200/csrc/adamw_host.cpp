@@ -28,6 +28,7 @@ namespace smo_host {
 namespace {
 
 using AdamwStepFn = int (*)(const smo_adamw_tensor *, int32_t, const float *, float, float *, void *, size_t, void *);
+using AdamwAdvanceFn = int (*)(const smo_adamw_schedule *, int32_t, smo_adamw_hyper *, void *);
 using AdamwDecodeFn = int (*)(const smo_adamw_tensor *, int32_t, void *);
 using GradNormFn = int (*)(const smo_grad *, int32_t, float, float *, void *, size_t, void *);
 using WorkspaceFn = size_t (*)(int32_t);
@@ -47,6 +48,8 @@ struct AdamEntry {
     void *held_ptr[kMaxKeys] = {};   // and the addresses the descriptor holds
     void *param_ptr = nullptr;
     std::vector<int64_t> sizes, strides;
+    PyObject *step = nullptr;        // owned: the state's step tensor (capturable plans)
+    float *step_ptr = nullptr;
     smo_adamw_tensor row;
 };
 
@@ -63,8 +66,11 @@ struct AdamPlan {
     int device = -1;
     int32_t rows = 0;
     AdamwStepFn step_fn = nullptr;
+    AdamwAdvanceFn advance_fn = nullptr;  // capturable: scalars are formed on the device
     unsigned long long generation = 0;
     std::vector<smo_adamw_tensor> table;
+    std::vector<smo_adamw_schedule> schedule;
+    std::vector<const float *> lr_dev;    // per group
     std::vector<long long> next_step;
     std::vector<double> hp_in;
 
@@ -72,6 +78,7 @@ struct AdamPlan {
         for (AdamEntry &e : entries) {
             Py_XDECREF(e.param);
             Py_XDECREF(e.state);
+            Py_XDECREF(e.step);
             for (PyObject *h : e.held) Py_XDECREF(h);
         }
         for (AdamGroup &g : groups) {
@@ -206,8 +213,34 @@ bool read_step(PyObject *state, long long *out) {
     return true;
 }
 
+// the state's step as an fp32 tensor of one element on the device, or null
+PyObject *step_tensor(PyObject *state, int device) {
+    PyObject *o = state_tensor(state, s_step);
+    if (!o) return nullptr;
+    const at::Tensor &t = THPVariable_Unpack(o);
+    const bool ok = t.is_cuda() && t.device().index() == device && t.scalar_type() == c10::ScalarType::Float &&
+                    t.numel() == 1 && t.layout() == c10::kStrided;
+    return ok ? o : nullptr;
+}
+
+// read_group() where the learning rate may be an fp32 tensor of one element on the device
+bool read_group_capturable(PyObject *g, int device, double *out, const float **lr_dev) {
+    PyObject *lr = PyDict_GetItemWithError(g, s_lr);
+    *lr_dev = nullptr;
+    if (!lr || !THPVariable_Check(lr)) return read_group(g, out);
+    const at::Tensor &t = THPVariable_Unpack(lr);
+    if (!t.is_cuda() || t.device().index() != device || t.scalar_type() != c10::ScalarType::Float || t.numel() != 1)
+        return false;
+    PyObject *plain = PyDict_Copy(g), *zero = PyFloat_FromDouble(0.0);
+    const bool ok = plain && zero && PyDict_SetItem(plain, s_lr, zero) == 0 && read_group(plain, out);
+    Py_XDECREF(plain);
+    Py_XDECREF(zero);
+    *lr_dev = (const float *)t.data_ptr();
+    return ok;
+}
+
 // null with no Python error: no plan for these parameters as they are
-PyObject *build_plan(PyObject *groups_list, PyObject *state_map, unsigned long long fn) {
+PyObject *build_plan(PyObject *groups_list, PyObject *state_map, unsigned long long fn, unsigned long long advance_fn) {
     AdamPlan *pl = new AdamPlan();
     PyObject *cap = PyCapsule_New(pl, "smo_adamw_plan", plan_free);
     if (!cap) {
@@ -221,6 +254,7 @@ PyObject *build_plan(PyObject *groups_list, PyObject *state_map, unsigned long l
     Py_INCREF(groups_list);
     pl->groups_list = groups_list;
     pl->step_fn = (AdamwStepFn)(uintptr_t)fn;
+    pl->advance_fn = (AdamwAdvanceFn)(uintptr_t)advance_fn;
     const Py_ssize_t ng = PyList_GET_SIZE(groups_list);
     pl->groups.resize(ng);
     for (Py_ssize_t gi = 0; gi < ng; gi++) {
@@ -247,9 +281,17 @@ PyObject *build_plan(PyObject *groups_list, PyObject *state_map, unsigned long l
             pl->device = p.device().index();
             PyObject *state = PyDict_GetItemWithError(state_map, param);
             long long step;
-            if (!state || !PyDict_Check(state) || !read_step(state, &step)) return none();
+            if (!state || !PyDict_Check(state)) return none();
             Py_INCREF(state);
             e.state = state;
+            if (pl->advance_fn) {
+                e.step = step_tensor(state, pl->device);
+                if (!e.step) return none();
+                Py_INCREF(e.step);
+                e.step_ptr = (float *)THPVariable_Unpack(e.step).data_ptr();
+            } else if (!read_step(state, &step)) {
+                return none();
+            }
             if (!fill_entry(e, p, g)) return none();
             pl->rows++;
         }
@@ -258,13 +300,16 @@ PyObject *build_plan(PyObject *groups_list, PyObject *state_map, unsigned long l
     if (g_watcher < 0 || PyDict_Watch(g_watcher, state_map) < 0) return none();
     pl->generation = g_state_generation;
     pl->table.resize(pl->rows);
+    if (pl->advance_fn) pl->schedule.resize(pl->rows);
+    pl->lr_dev.resize(ng);
     pl->next_step.resize(pl->entries.size());
     pl->hp_in.resize(5 * ng);
     return cap;
 }
 
 // -2: a Python error is set; -1: the plan does not apply (nothing modified); 0: stepped; > 0: smo_status
-int run_plan(AdamPlan &pl, const float *scale, float max_norm, float *norm_out, void *ws, size_t ws_bytes) {
+int run_plan(AdamPlan &pl, const float *scale, float max_norm, float *norm_out, void *ws, size_t ws_bytes,
+             smo_adamw_hyper *hypers) {
     if (pl.generation != g_state_generation) return -1;
     if (!PyList_CheckExact(pl.groups_list) || PyList_GET_SIZE(pl.groups_list) != (Py_ssize_t)pl.groups.size())
         return -1;
@@ -276,7 +321,9 @@ int run_plan(AdamPlan &pl, const float *scale, float max_norm, float *norm_out, 
         if (ps != g.params || PyList_GET_SIZE(ps) != g.n) return -1;
         for (Py_ssize_t j = 0; j < g.n; j++, k++)
             if (PyList_GET_ITEM(ps, j) != pl.entries[k].param) return -1;
-        if (!read_group(g.dict, &pl.hp_in[5 * gi])) return -1;
+        if (pl.advance_fn ? !read_group_capturable(g.dict, pl.device, &pl.hp_in[5 * gi], &pl.lr_dev[gi])
+                          : !read_group(g.dict, &pl.hp_in[5 * gi]))
+            return -1;
     }
     size_t m = 0;
     int last_group = -1;
@@ -299,26 +346,38 @@ int run_plan(AdamPlan &pl, const float *scale, float max_norm, float *norm_out, 
                 return -1;
         // a moment or a master copy that came or went makes another kind of entry
         if (PyDict_GET_SIZE(e.state) != e.nstate) return -1;
-        long long step;
-        if (!read_step(e.state, &step)) return -1;
-        pl.next_step[i] = ++step;
-        if (e.group != last_group || step != last_step) {
-            hp = make_hyper(&pl.hp_in[5 * e.group], step);
-            last_group = e.group;
-            last_step = step;
-        }
-        smo_adamw_tensor &r = pl.table[m++];
+        smo_adamw_tensor &r = pl.table[m];
         r = e.row;
         r.grad = g.data_ptr();
-        r.hp = hp;
+        if (pl.advance_fn) {
+            if (PyDict_GetItemWithError(e.state, s_step) != e.step ||
+                THPVariable_Unpack(e.step).data_ptr() != e.step_ptr)
+                return -1;
+            const double *in = &pl.hp_in[5 * e.group];
+            pl.schedule[m] = smo_adamw_schedule{e.step_ptr, pl.lr_dev[e.group], in[0], in[1], in[2], in[3], in[4]};
+            r.hp_dev = hypers + m;
+        } else {
+            long long step;
+            if (!read_step(e.state, &step)) return -1;
+            pl.next_step[i] = ++step;
+            if (e.group != last_group || step != last_step) {
+                hp = make_hyper(&pl.hp_in[5 * e.group], step);
+                last_group = e.group;
+                last_step = step;
+            }
+            r.hp = hp;
+        }
+        m++;
     }
-    int rc;
+    int rc = SMO_OK;
     {
         c10::cuda::CUDAGuard guard((c10::DeviceIndex)pl.device);
         cudaStream_t stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)pl.device).stream();
+        if (pl.advance_fn) rc = pl.advance_fn(pl.schedule.data(), (int32_t)m, hypers, (void *)stream);
+        if (rc != SMO_OK) return rc;
         rc = pl.step_fn(pl.table.data(), (int32_t)m, scale, max_norm, norm_out, ws, ws_bytes, (void *)stream);
     }
-    if (rc != SMO_OK) return rc;
+    if (rc != SMO_OK || pl.advance_fn) return rc;
     for (size_t i = 0; i < pl.entries.size(); i++) {
         if (!pl.entries[i].state) continue;
         PyObject *ns = PyLong_FromLongLong(pl.next_step[i]);
@@ -344,13 +403,15 @@ bool adamw_init() {
     return s_exp_avg && s_exp_avg_sq && s_m_q && s_m_s && s_v_q && s_v_s && s_master;
 }
 
-// adamw_plan(param_groups, state_mapping, step_fn_addr) -> (capsule, device index, tensors) or None
+// adamw_plan(param_groups, state_mapping, step_fn_addr, advance_fn_addr) -> (capsule, device index, tensors) or
+// None; advance_fn_addr is 0 unless the step counts are device tensors
 PyObject *adamw_plan(PyObject *, PyObject *args) {
     PyObject *groups_list, *state_map;
-    unsigned long long fn;
-    if (!PyArg_ParseTuple(args, "O!O!K", &PyList_Type, &groups_list, &PyDict_Type, &state_map, &fn)) return nullptr;
+    unsigned long long fn, advance_fn;
+    if (!PyArg_ParseTuple(args, "O!O!KK", &PyList_Type, &groups_list, &PyDict_Type, &state_map, &fn, &advance_fn))
+        return nullptr;
     try {
-        PyObject *cap = build_plan(groups_list, state_map, fn);
+        PyObject *cap = build_plan(groups_list, state_map, fn, advance_fn);
         if (!cap) {
             PyErr_Clear();
             Py_RETURN_NONE;
@@ -363,17 +424,18 @@ PyObject *adamw_plan(PyObject *, PyObject *args) {
     }
 }
 
-// adamw_run(capsule, grad_scale address or 0, max_norm or 0, norm address or 0, workspace address, bytes)
+// adamw_run(capsule, address of the scalars' device memory or 0, grad_scale address or 0, max_norm or 0, norm
+// address or 0, workspace address, bytes)
 PyObject *adamw_run(PyObject *, PyObject *args) {
     PyObject *cap;
-    unsigned long long scale, norm_out, ws, ws_bytes;
+    unsigned long long hypers, scale, norm_out, ws, ws_bytes;
     float max_norm;
-    if (!PyArg_ParseTuple(args, "OKfKKK", &cap, &scale, &max_norm, &norm_out, &ws, &ws_bytes)) return nullptr;
+    if (!PyArg_ParseTuple(args, "OKKfKKK", &cap, &hypers, &scale, &max_norm, &norm_out, &ws, &ws_bytes)) return nullptr;
     AdamPlan *pl = (AdamPlan *)PyCapsule_GetPointer(cap, "smo_adamw_plan");
     if (!pl) return nullptr;
     try {
         const int rc = run_plan(*pl, (const float *)(uintptr_t)scale, max_norm, (float *)(uintptr_t)norm_out,
-                                (void *)(uintptr_t)ws, (size_t)ws_bytes);
+                                (void *)(uintptr_t)ws, (size_t)ws_bytes, (smo_adamw_hyper *)(uintptr_t)hypers);
         if (rc == -2) return nullptr;
         PyErr_Clear();
         return PyLong_FromLong(rc);

@@ -6,6 +6,7 @@ import ctypes
 import numpy as np
 import pytest
 import torch
+from torch.optim.optimizer import register_optimizer_step_post_hook
 
 from smo_optimizer_b200 import AdamW, AdamW8bit, _host, _lib, clip_grad_norm_, grad_norm
 from smo_optimizer_b200.optimizers import _host_ext
@@ -22,6 +23,13 @@ def _p(n=10, dtype=torch.float32):
 def test_constructor_refusals(cls, bad):
     with pytest.raises(ValueError, match="Invalid"):
         cls([_p()], **bad)
+
+
+@pytest.mark.parametrize("cls", [AdamW, AdamW8bit])
+def test_lr_as_a_tensor_needs_capturable(cls):
+    with pytest.raises(ValueError, match="capturable"):
+        cls([_p()], lr=torch.tensor(1e-3))
+    assert cls([_p()], lr=torch.tensor(1e-3), capturable=True).capturable
 
 
 def test_constructor_refusals_of_8bit():
@@ -166,7 +174,7 @@ def test_step_hooks_and_schedulers(cls):
     seen = []
     handles = [opt.register_step_pre_hook(lambda o, args, kw: seen.append("pre")),
                opt.register_step_post_hook(lambda o, args, kw: seen.append("post")),
-               torch.optim.optimizer.register_optimizer_step_post_hook(lambda o, args, kw: seen.append("all"))]
+               register_optimizer_step_post_hook(lambda o, args, kw: seen.append("all"))]
     opt.step()
     assert seen == ["pre", "post", "all"] or sorted(seen) == ["all", "post", "pre"]
     for h in handles:
@@ -181,3 +189,15 @@ def test_step_hooks_and_schedulers(cls):
     opt.step()
     sched.step()
     assert opt.param_groups[0]["lr"] == 0.25
+
+
+def test_schedules_are_validated():
+    lib = _lib.load()
+    t = np.zeros(1, dtype=_lib.SCHEDULE_DTYPE)
+    assert _lib.SCHEDULE_DTYPE.itemsize == 56
+    advance = lambda n=1, out=1 << 20: lib.smo_adamw_advance(t.ctypes.data, n, out, None)  # noqa: E731
+    assert advance(n=0) == 0 and advance(n=-1) == 1 and advance() == 1   # no step count
+    t["step"] = 1 << 21
+    assert advance(out=None) == 1 and advance(out=2) == 2
+    t["step"] = 2
+    assert advance() == 2

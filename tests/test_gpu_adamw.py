@@ -604,6 +604,95 @@ def test_capture_with_host_scalars_is_refused():
     assert opt.state[params[0]]["step"] == 2 and not torch.equal(before, params[0].detach())
 
 
+@pytest.mark.parametrize("cls", [AdamW, AdamW8bit])
+def test_capturable_steps_give_the_same_bits(cls):
+    """Scalars formed on the device, with the learning rate as a number and as a tensor, through the C++ and the
+    Python path."""
+    made = []
+    for kw in (dict(), dict(capturable=True), dict(capturable=True, lr=torch.tensor(HP["lr"], device="cuda")),
+               dict(capturable=True)):
+        params = _params([5000, 30, 2049], torch.bfloat16)
+        made.append((params, cls(params, **dict(HP, max_grad_norm=0.1, **kw))))
+    for step in range(5):
+        for k, (params, o) in enumerate(made):
+            _grads(params, step)
+            if k == 3:
+                o._slow_step(o._ready(), None)
+            else:
+                o.step()
+    (pa, a), rest = made[0], made[1:]
+    for pb, b in rest:
+        for p, q in zip(pa, pb):
+            assert torch.equal(p.detach(), q.detach())
+            assert float(b.state[q]["step"]) == a.state[p]["step"] == 5
+            for k, t in a.state[p].items():
+                assert not torch.is_tensor(t) or torch.equal(t, b.state[q][k]), k
+    # either kind loads the other's state
+    c = cls(pa, **HP)
+    c.load_state_dict(rest[0][1].state_dict())
+    assert c.state[pa[0]]["step"] == 5 and type(c.state[pa[0]]["step"]) is int
+    d = cls(pa, capturable=True, **HP)
+    d.load_state_dict(a.state_dict())
+    assert float(d.state[pa[0]]["step"]) == 5.0 and d.state[pa[0]]["step"].is_cuda
+
+
+@pytest.mark.parametrize("cls", [AdamW, AdamW8bit])
+def test_captured_step_replays(cls):
+    """A captured step, replayed with new gradients and a new learning rate, against eager steps; eager steps in
+    between and a second graph of the same optimizer."""
+    lr = torch.tensor(HP["lr"], device="cuda")
+    sizes = [5000, 30, 2049]
+    params, plain = _params(sizes, torch.float32), _params(sizes, torch.float32)
+    kw = dict(HP, max_grad_norm=0.1)
+    opt, ref = cls(params, capturable=True, **dict(kw, lr=lr)), cls(plain, **kw)
+    _grads(params, 0)
+    _grads(plain, 0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opt.step()
+    torch.cuda.current_stream().wait_stream(side)
+    ref.step()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for g in graphs:
+        with torch.cuda.graph(g):
+            opt.step()
+    for step in range(1, 7):
+        r = _rng(step)
+        for p, q in zip(params, plain):
+            q.grad = torch.from_numpy(r.normal(0, 1e-2, tuple(p.shape)).astype(np.float32)).cuda()
+            p.grad.copy_(q.grad)
+        value = HP["lr"] / step
+        lr.fill_(value)
+        ref.param_groups[0]["lr"] = float(lr)  # the fp32 number that the device reads
+        if step == 4:
+            opt.step()
+        else:
+            graphs[step % 2].replay()
+        ref.step()
+        assert torch.equal(opt.last_grad_norm, ref.last_grad_norm), step
+        for p, q in zip(params, plain):
+            assert torch.equal(p.detach(), q.detach()), step
+            assert float(opt.state[p]["step"]) == ref.state[q]["step"] == step + 1
+            for k, t in ref.state[q].items():
+                assert not torch.is_tensor(t) or torch.equal(t, opt.state[p][k]), (k, step)
+
+
+def test_first_step_in_a_capture_is_refused():
+    params = _params([300], torch.float32)
+    opt = AdamW(params, capturable=True, **HP)
+    _grads(params, 1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="first step"):
+            opt.step()
+    assert not opt.state[params[0]]
+    opt.step()
+    with pytest.raises(TypeError, match="lr"):
+        opt.param_groups[0]["lr"] = torch.tensor(1e-3, dtype=torch.float64, device="cuda")
+        opt.step()
+
+
 def test_launches_are_counted():
     params = _params([300, 5000], torch.float32)
     opt = AdamW(params, **HP)
