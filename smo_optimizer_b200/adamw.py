@@ -11,7 +11,8 @@ model their rounding.  The arithmetic is stated in include/smo_b200.h
 
 As with the other optimizers here the parameters are CUDA tensors (fp32, bf16
 or fp16) with gradients of their own type, the work runs on the current stream,
-and there is no CPU path.
+and there is no CPU path.  All tensors of a step are written in one launch or in
+launches that overlap: they must not share memory.
 """
 
 from __future__ import annotations
@@ -58,9 +59,10 @@ def _norm(parameters, max_norm, what):
 
 @torch.no_grad()
 def _norm_of_copies(parameters, max_norm, what, ext, fn, ws):
-    """Refusals, no gradients at all (None), and gradients with gaps or repeated
-    elements: those are taken as copies, written back when clipped."""
-    grads = [p.grad for p in parameters if p.grad is not None]
+    """Refusals, no gradients at all (None), parameters given twice (taken once),
+    and gradients with gaps or repeated elements: those are taken as copies,
+    written back when clipped."""
+    grads = [p.grad for p in {id(p): p for p in parameters}.values() if p.grad is not None]
     for g in grads:
         if g.is_sparse:
             raise RuntimeError(f"{what} does not support sparse gradients.")
@@ -78,6 +80,8 @@ def _norm_of_copies(parameters, max_norm, what, ext, fn, ws):
         holder.grad = g.contiguous()
         holders.append(holder)
     got = ext.grad_norm(holders, max_norm, fn, ws)
+    if got is None:
+        raise RuntimeError(f"{what}: two parameters share one gradient")
     if max_norm > 0:
         for g, h in zip(grads, holders):
             if h.grad.data_ptr() != g.data_ptr():
@@ -92,7 +96,8 @@ def grad_norm(parameters) -> torch.Tensor:
     Parameters without a gradient are left out.  Each gradient is read once;
     squares and sums are held in double, in an order that depends on the sizes
     alone, so the same gradients always give the same bits.  Nothing
-    synchronises.  Without any gradient: 0, on the CPU."""
+    synchronises.  A parameter given twice counts once.  Without any gradient:
+    0, on the CPU."""
     return _norm(parameters, 0.0, "grad_norm")
 
 
@@ -157,6 +162,15 @@ class _AdamWBase(Optimizer):
         self._workspace, self._scalars = {}, {}
         self._kept = getattr(self, "_kept", [])
         self.last_grad_norm = None
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        # torch only warns of a parameter that a group holds twice; stepped in one
+        # launch, the two would write the same memory
+        params = self.param_groups[-1]["params"]
+        if len(set(map(id, params))) < len(params):
+            self.param_groups.pop()
+            raise ValueError("a parameter appears more than once in a parameter group")
 
     def _eight_bit(self, p, group) -> bool:
         return False
@@ -471,7 +485,7 @@ class AdamW(_AdamWBase):
     ``max_grad_norm``: scale the gradients of each step by
     ``min(1, max_grad_norm / (norm + 1e-6))`` within the step;
     ``last_grad_norm`` is then the norm (a device tensor, overwritten by the next
-    step).
+    step).  As with ``clip_grad_norm_`` a norm that is NaN makes the step NaN.
     ``capturable``: the step can be captured into a CUDA graph and replayed.  The
     step counts are then fp32 device tensors and the scalars are formed on the
     device (one more launch); ``lr`` may be an fp32 device tensor, which replays

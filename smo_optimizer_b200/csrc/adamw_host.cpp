@@ -11,6 +11,7 @@
 
 #include "smo_host.h"
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstring>
@@ -338,6 +339,7 @@ int run_plan(AdamPlan &pl, const float *scale, float max_norm, float *norm_out, 
             continue;
         }
         if (!g.defined() || p.data_ptr() != e.param_ptr) return -1;
+        if (dtype_code(p.scalar_type()) != e.row.dtype || p.device().index() != pl.device) return -1;
         if (p.sizes() != c10::IntArrayRef(e.sizes) || p.strides() != c10::IntArrayRef(e.strides)) return -1;
         if (g.scalar_type() != p.scalar_type() || !same_layout(p, g)) return -1;
         for (int q = 0; q < e.nkeys; q++)
@@ -512,7 +514,8 @@ PyObject *adamw_moments(PyObject *, PyObject *args) {
 }
 
 // grad_norm([parameter], max_norm, norm_fn_addr, workspace_fn_addr) -> (status, norm tensor), or None where a
-// gradient is not on the first one's CUDA device, of a known type and one span of memory, or there is none
+// gradient is not on the first one's CUDA device, of a known type and one span of memory, is there twice, or there is
+// none
 PyObject *grad_norm(PyObject *, PyObject *args) {
     PyObject *list;
     float max_norm;
@@ -536,6 +539,13 @@ PyObject *grad_norm(PyObject *, PyObject *args) {
             table.push_back(smo_grad{g.data_ptr(), g.numel(), dt, 0});
         }
         if (device < 0) Py_RETURN_NONE;
+        // a parameter given twice would be counted, and scaled, twice
+        std::vector<uintptr_t> seen;
+        seen.reserve(table.size());
+        for (const smo_grad &g : table)
+            if (g.n) seen.push_back((uintptr_t)g.grad);
+        std::sort(seen.begin(), seen.end());
+        if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) Py_RETURN_NONE;
         c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
         const size_t bytes = ((WorkspaceFn)(uintptr_t)ws_fn)((int32_t)table.size());
         const auto on = at::TensorOptions().device(c10::Device(c10::kCUDA, (c10::DeviceIndex)device));

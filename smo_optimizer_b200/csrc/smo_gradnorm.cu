@@ -142,12 +142,6 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__
 
 // ---------------------------------------------------------------- host side
 
-int cuda_status(cudaError_t e) {
-    if (e == cudaSuccess) return SMO_OK;
-    g_last_cuda_error = (int)e;
-    return SMO_ERR_CUDA;
-}
-
 // launches over n tensors: full batches, and up to one more for each dtype
 int32_t most_launches(int32_t n) { return n / kCap + 3; }
 

@@ -96,6 +96,15 @@ __device__ __forceinline__ void st8_part(T *p, int64_t left, const float (&x)[8]
         if (k < left) st<T>(p + k, x[k]);
 }
 
+// the status of a CUDA call; an error is taken from the runtime, so that it is not
+// blamed on a later call
+inline int cuda_status(cudaError_t e) {
+    if (e == cudaSuccess) return SMO_OK;
+    g_last_cuda_error = (int)e;
+    (void)cudaGetLastError();
+    return SMO_ERR_CUDA;
+}
+
 inline bool is_aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
 inline size_t dtype_bytes(int32_t dtype) { return dtype == SMO_DTYPE_F32 ? 4 : 2; }
 inline bool known_dtype(int32_t dtype) {

@@ -45,6 +45,19 @@ def test_constructor_refusals_of_8bit():
 
 
 @pytest.mark.parametrize("cls", [AdamW, AdamW8bit])
+def test_a_parameter_given_twice_is_refused(cls):
+    p, q = _p(), _p()
+    with pytest.warns(UserWarning), pytest.raises(ValueError, match="more than once"):
+        cls([p, p])
+    opt = cls([p])
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": [p]})
+    with pytest.warns(UserWarning), pytest.raises(ValueError, match="more than once"):
+        opt.add_param_group({"params": [q, q]})
+    assert len(opt.param_groups) == 1
+
+
+@pytest.mark.parametrize("cls", [AdamW, AdamW8bit])
 def test_step_refusals(cls):
     p = _p()
     opt = cls([p])
@@ -201,3 +214,15 @@ def test_schedules_are_validated():
     assert advance(out=None) == 1 and advance(out=2) == 2
     t["step"] = 2
     assert advance() == 2
+
+
+def test_zero1_refuses_a_norm_of_one_ranks_gradients(monkeypatch):
+    from smo_optimizer_b200 import zero
+
+    monkeypatch.setattr(zero.dist, "is_initialized", lambda: True)
+    monkeypatch.setattr(zero.dist, "get_world_size", lambda group=None: 2)
+    monkeypatch.setattr(zero.dist, "get_rank", lambda group=None: 0)
+    with pytest.raises(ValueError, match="max_grad_norm"):
+        zero.Zero1([_p(), _p()], AdamW, max_grad_norm=1.0)
+    z = zero.Zero1([_p(100), _p(200), _p(90)], AdamW8bit, min_8bit_numel=0, block_size=64)
+    assert z.owner == [1, 0, 1] and z.costs[1] == adamw_step_bytes((200,), True, 64, 0)

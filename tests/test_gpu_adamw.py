@@ -693,6 +693,36 @@ def test_first_step_in_a_capture_is_refused():
         opt.step()
 
 
+def test_grad_scaler_and_closure():
+    params, plain = _params([3000, 7], torch.float32), _params([3000, 7], torch.float32)
+    opt, ref = AdamW8bit(params, min_8bit_numel=0, **HP), AdamW8bit(plain, min_8bit_numel=0, **HP)
+    scaler = torch.amp.GradScaler("cuda", init_scale=8.0)
+    _grads(plain, 1)
+    for p, q in zip(params, plain):
+        p.grad = q.grad * 8.0
+    scaler.scale(torch.zeros((), device="cuda"))
+    scaler.step(opt)
+    scaler.update()
+    ref.step()
+    assert all(torch.equal(p.detach(), q.detach()) for p, q in zip(params, plain))
+    params[0].grad = torch.full_like(params[0], float("inf"))
+    before = params[1].detach().clone()
+    scaler.step(opt)  # skipped
+    assert torch.equal(params[1].detach(), before) and opt.state[params[0]]["step"] == 1
+
+    def closure():
+        opt.zero_grad()
+        loss = sum((p * p).sum() for p in params)
+        loss.backward()
+        return loss
+
+    loss = opt.step(closure)
+    assert loss.requires_grad and opt.state[params[0]]["step"] == 2
+    opt.zero_grad()
+    opt.step()
+    assert opt.state[params[0]]["step"] == 2
+
+
 def test_launches_are_counted():
     params = _params([300, 5000], torch.float32)
     opt = AdamW(params, **HP)

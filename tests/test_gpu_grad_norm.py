@@ -141,3 +141,19 @@ def test_captured_norm_and_clip_replay():
         want = clip_grad_norm_(fresh, 1.0)
         assert torch.equal(norm, want)
         assert all(torch.equal(p.grad, q.grad) for p, q in zip(params, fresh))
+
+
+def test_a_parameter_given_twice_counts_once():
+    params = _set([5000, 300], [torch.float32])
+    want = _exact(params)
+    kept = [p.grad.clone() for p in params]
+    twice = params + [params[0]]
+    assert _close(grad_norm(twice), want)
+    norm = clip_grad_norm_(twice, 0.5)
+    c = torch.tensor(0.5, device="cuda") / (norm + 1e-6)
+    for p, g in zip(params, kept):
+        assert torch.equal(p.grad, g * c)
+    other = torch.nn.Parameter(torch.zeros(5000, device="cuda"))
+    other.grad = params[0].grad
+    with pytest.raises(RuntimeError, match="share"):
+        grad_norm(params + [other])
