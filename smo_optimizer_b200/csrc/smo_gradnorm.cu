@@ -59,6 +59,7 @@ __device__ __forceinline__ double cta_sum(double x) {
 
 template <class T, int CAP>
 __global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__ GradBatch<CAP> b) {
+    wait_for_previous();
     let_next_start();
     const int32_t total = b.start[b.n];
     double acc = 0.0;
@@ -98,7 +99,9 @@ struct NormArgs {
 
 // norm = sqrt(sum of the parts) * |scale|; coef = min(1, max_norm / (norm + 1e-6)) * scale
 __global__ void __launch_bounds__(kSumThreads) norm_kernel(NormArgs a) {
-    let_next_start();
+    // the step or scaling that uses the factor may start: everything in front of the
+    // partial sums had ended when those let this kernel start
+    if (a.max_norm > 0.0f && a.n > 0) let_next_start();
     wait_for_previous();
     double acc = 0.0;
     for (int32_t i = threadIdx.x; i < a.n; i += kSumThreads) acc += a.part[i];
@@ -150,10 +153,10 @@ int launch(const GradBatch<CAP> &b, int32_t &parts, cudaStream_t s) {
     const int32_t chunks = b.start[b.n];
     cudaError_t e;
     if (b.coef) {
-        e = launch_batch(scale_kernel<T, CAP>, (unsigned)chunks, kThreads, b, true, s);
+        e = launch_batch(scale_kernel<T, CAP>, (unsigned)chunks, kThreads, b, s);
     } else {
         const int32_t ctas = chunks < kParts ? chunks : kParts;
-        e = launch_batch(sumsq_kernel<T, CAP>, (unsigned)ctas, kThreads, b, false, s);
+        e = launch_batch(sumsq_kernel<T, CAP>, (unsigned)ctas, kThreads, b, s);
         parts += ctas;
     }
     g_launches++;
@@ -228,10 +231,8 @@ int grad_norm_enqueue(GradOf grad_of, const void *items, int32_t n, const float 
     int32_t parts = 0;
     const int st = run(grad_of, items, n, part, nullptr, parts, s);
     if (st != SMO_OK) return st;
-    // it may start early only behind a partial sum, which itself started after
-    // everything before it had ended
-    const cudaError_t e = launch_batch(norm_kernel, 1, kSumThreads, NormArgs{part, parts, scale, max_norm, norm_out, coef},
-                                       parts > 0, s);
+    const cudaError_t e =
+        launch_batch(norm_kernel, 1, kSumThreads, NormArgs{part, parts, scale, max_norm, norm_out, coef}, s);
     g_launches++;
     if (coef_out) *coef_out = coef;
     return cuda_status(e);

@@ -20,12 +20,13 @@ namespace smo {
 // 32,764 bytes is the most that one launch's parameters may hold
 constexpr size_t kMaxParamBytes = 32764;
 
-// Launch of a kernel whose one parameter is the batch.  `after`: it may start
-// while the kernel before it in the stream ends (programmatic dependent
-// launch); it then calls wait_for_previous() before it reads that kernel's results
-// or writes what that kernel reads.
+// Launch of a kernel whose one parameter is the batch, as a programmatic
+// dependent launch: its CTAs may start while the kernel in front of it in the
+// stream ends (2 us less between two kernels).  So every kernel launched this way
+// calls wait_for_previous() before it touches memory that anything in front of it
+// may touch.
 template <class B>
-cudaError_t launch_batch(void (*kernel)(B), unsigned ctas, unsigned threads, const B &b, bool after, cudaStream_t s) {
+cudaError_t launch_batch(void (*kernel)(B), unsigned ctas, unsigned threads, const B &b, cudaStream_t s) {
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
@@ -34,13 +35,16 @@ cudaError_t launch_batch(void (*kernel)(B), unsigned ctas, unsigned threads, con
     cfg.blockDim = dim3(threads);
     cfg.stream = s;
     cfg.attrs = &attr;
-    cfg.numAttrs = after ? 1 : 0;
+    cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, b);
 }
 
 // every kernel before this one in the stream has ended and its writes are visible
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-// the next kernel may start as soon as every CTA has come here (or ended)
+// The next kernel may start as soon as every CTA has come here (or ended).  Only
+// where that is a kernel of this library that knows what it may read before it
+// waits, and only once everything in front has ended: after wait_for_previous(),
+// or in a kernel that could itself start early for that reason.
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // index of the tensor that holds chunk `c`: the last i with start[i] <= c

@@ -678,6 +678,45 @@ def test_captured_step_replays(cls):
                 assert not torch.is_tensor(t) or torch.equal(t, opt.state[p][k]), (k, step)
 
 
+def test_captured_behind_copies_and_joined_streams():
+    """What comes before the calls in a graph may be a copy, a fill, or work joined from another stream."""
+    params, plain = _params([70000, 300], torch.bfloat16), _params([70000, 300], torch.bfloat16)
+    kw = dict(HP, master_weights=True)
+    opt, ref = AdamW8bit(params, capturable=True, **kw), AdamW8bit(plain, **kw)
+    _grads(params, 0)
+    _grads(plain, 0)
+    opt.step()
+    ref.step()
+    fresh = [torch.zeros_like(p) for p in params]
+    out = [tuple(torch.zeros(p.shape, device="cuda") for _ in range(2)) for p in params]
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            params[1].grad.copy_(fresh[1])  # a copy on another stream
+        params[0].grad.zero_()  # a fill
+        main.wait_stream(side)
+        grad_norm(params)
+        params[0].grad.copy_(fresh[0])
+        clip_grad_norm_(params, 0.5)
+        opt.step()
+        opt.moments(params, out=out)
+    for step in range(1, 6):
+        _grads(plain, step, scale=0.1)
+        for f, q in zip(fresh, plain):
+            f.copy_(q.grad)
+        graph.replay()
+        clip_grad_norm_(plain, 0.5)
+        ref.step()
+        want = ref.moments(plain)
+        for p, q, a, b in zip(params, plain, out, want):
+            assert torch.equal(p.grad, q.grad) and torch.equal(p.detach(), q.detach()), step
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]), step
+
+
 def test_first_step_in_a_capture_is_refused():
     params = _params([300], torch.float32)
     opt = AdamW(params, capturable=True, **HP)
