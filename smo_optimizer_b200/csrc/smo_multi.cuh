@@ -86,20 +86,6 @@ __device__ __forceinline__ void st8(T *p, const float (&x)[8]) {
     }
 }
 
-// The first `left` (at most 8) of eight consecutive elements; 0 behind them.
-template <class T>
-__device__ __forceinline__ void ld8_part(const T *p, int64_t left, float (&x)[8]) {
-#pragma unroll
-    for (int k = 0; k < 8; k++) x[k] = k < left ? ld<T>(p + k) : 0.0f;
-}
-
-template <class T>
-__device__ __forceinline__ void st8_part(T *p, int64_t left, const float (&x)[8]) {
-#pragma unroll
-    for (int k = 0; k < 8; k++)
-        if (k < left) st<T>(p + k, x[k]);
-}
-
 // the status of a CUDA call; an error is taken from the runtime, so that it is not
 // blamed on a later call
 inline int cuda_status(cudaError_t e) {

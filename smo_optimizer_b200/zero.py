@@ -205,8 +205,8 @@ class Zero1:
         self.rank = dist.get_rank(process_group) if dist.is_initialized() else 0
         self.params = [p for p in params]
         if self.world > 1 and kwargs.get("max_grad_norm") is not None:
-            raise ValueError("max_grad_norm: a rank's optimizer sees the gradients of its own tensors only; "
-                             "clip before Zero1.step()")
+            raise ValueError("max_grad_norm: a rank's optimizer sees the gradients of its own tensors only; gradients "
+                             "that every rank holds whole can be clipped before Zero1.step()")
         costs = [_step_cost(p, optimizer_cls, kwargs) for p in self.params]
         self.owner = lpt_partition(costs, self.world)
         self.costs = costs
