@@ -205,14 +205,15 @@ class _AdamWBase(Optimizer):
                     raise TypeError(f"{self._name} (B200 build) steps fp32, bf16 or fp16 parameters with "
                                     f"gradients of the same dtype; got {p.dtype} / {grad.dtype}")
                 state = self.state[p]
+                master = self.master_weights and p.dtype != torch.float32 and "master" not in state
+                if ("step" not in state or master) and torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError(f"{self._name}: the first step of a parameter cannot be captured (replays would "
+                                       "make its state anew); take one before the capture")
                 if "step" not in state:
-                    if torch.cuda.is_current_stream_capturing():
-                        raise RuntimeError(f"{self._name}: the first step of a parameter cannot be captured (replays "
-                                           "would make its state anew); take one before the capture")
                     self._init_state(p, group)
-                state["step"] = self._step_value(p, state["step"])
-                if self.master_weights and p.dtype != torch.float32 and "master" not in state:
+                if master:
                     state["master"] = p.detach().to(torch.float32, memory_format=torch.preserve_format)
+                state["step"] = self._step_value(p, state["step"])
                 found.append((p, grad, state, group))
         return found
 
@@ -403,6 +404,8 @@ class _AdamWBase(Optimizer):
                                                        _stream(dev)))
                 for dst, src in back:
                     dst.copy_(src)
+            # autograd sees that the parameters were written
+            torch.autograd.graph.increment_version([p for p, _, _, _ in items])
             if not self.capturable:
                 for p, grad, state, group in items:
                     state["step"] += 1

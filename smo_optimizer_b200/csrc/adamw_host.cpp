@@ -379,7 +379,11 @@ int run_plan(AdamPlan &pl, const float *scale, float max_norm, float *norm_out, 
         if (rc != SMO_OK) return rc;
         rc = pl.step_fn(pl.table.data(), (int32_t)m, scale, max_norm, norm_out, ws, ws_bytes, (void *)stream);
     }
-    if (rc != SMO_OK || pl.advance_fn) return rc;
+    if (rc != SMO_OK) return rc;
+    // autograd sees that the parameters were written
+    for (const AdamEntry &e : pl.entries)
+        if (e.state) THPVariable_Unpack(e.param).unsafeGetTensorImpl()->bump_version();
+    if (pl.advance_fn) return SMO_OK;
     for (size_t i = 0; i < pl.entries.size(); i++) {
         if (!pl.entries[i].state) continue;
         PyObject *ns = PyLong_FromLongLong(pl.next_step[i]);
@@ -554,6 +558,11 @@ PyObject *grad_norm(PyObject *, PyObject *args) {
         cudaStream_t stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
         const int rc = ((GradNormFn)(uintptr_t)fn)(table.data(), (int32_t)table.size(), max_norm, (float *)out.data_ptr(),
                                                    ws.data_ptr(), bytes, (void *)stream);
+        if (rc == SMO_OK && max_norm > 0.0f)
+            for (Py_ssize_t i = 0; i < n; i++) {
+                const at::Tensor &g = THPVariable_Unpack(PyList_GET_ITEM(list, i)).grad();
+                if (g.defined()) g.unsafeGetTensorImpl()->bump_version();
+            }
         return Py_BuildValue("iN", rc, THPVariable_Wrap(out));
     } catch (const std::exception &e) {
         PyErr_SetString(PyExc_RuntimeError, e.what());

@@ -727,9 +727,83 @@ def test_first_step_in_a_capture_is_refused():
             opt.step()
     assert not opt.state[params[0]]
     opt.step()
+    half = _params([300], torch.bfloat16)
+    opt2 = AdamW(half, capturable=True, **HP)
+    _grads(half, 1)
+    opt2.step()
+    opt2.master_weights = True
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(RuntimeError, match="first step"):
+            opt2._plan = None
+            opt2.step()
+    assert "master" not in opt2.state[half[0]]
     with pytest.raises(TypeError, match="lr"):
         opt.param_groups[0]["lr"] = torch.tensor(1e-3, dtype=torch.float64, device="cuda")
         opt.step()
+
+
+@pytest.mark.parametrize("block", [None, 64])
+def test_master_copies_beside_fp32_parameters(block):
+    """fp32 and half-precision parameters in one optimizer with master copies, a scalar and odd sizes among them."""
+    shapes = [(), (3, 700), (1,), (4099,), (17, 5, 3)]
+    r = _rng(12)
+    params = [torch.nn.Parameter(torch.from_numpy(np.asarray(r.normal(0, 0.1, s), np.float32)).cuda().to(t))
+              for t in TYPES for s in shapes]
+    kw = dict(HP, master_weights=True)
+    opt = AdamW(params, **kw) if block is None else AdamW8bit(params, block_size=block, min_8bit_numel=0, **kw)
+    refs = [Plain32(_np(p), block) for p in params]
+    for step in range(3):
+        _grads(params, 40 + step)
+        opt.step()
+        for p, ref in zip(params, refs):
+            ref.step(_np(p.grad), *ARGS)
+    for p, ref in zip(params, refs):
+        st = opt.state[p]
+        assert ("master" in st) == (p.dtype != torch.float32)
+        _check_param(_np(st.get("master", p)), ref, (p.dtype, p.shape))
+        assert torch.equal(p.detach(), st.get("master", p).to(p.dtype).detach())
+        if block:
+            _check_codes(st, ref, (p.dtype, p.shape))
+
+
+def test_refused_types_and_gradients():
+    p = torch.nn.Parameter(torch.zeros(8, dtype=torch.float64, device="cuda"))
+    p.grad = torch.zeros_like(p)
+    with pytest.raises(TypeError, match="fp32, bf16 or fp16"):
+        AdamW([p]).step()
+    with pytest.raises(TypeError, match="fp32, bf16 or fp16"):
+        grad_norm([p])
+    q = torch.nn.Parameter(torch.zeros(8, device="cuda"))
+    q.grad = torch.zeros_like(q)
+    c = torch.nn.Parameter(torch.zeros(8))
+    c.grad = torch.zeros(8)
+    for params in ([q, c], [c, q]):
+        with pytest.raises(RuntimeError, match="CUDA tensors only"):
+            AdamW8bit(params).step()
+        with pytest.raises(RuntimeError, match="CUDA tensors only"):
+            clip_grad_norm_(params, 1.0)
+
+
+@pytest.mark.parametrize("slow", [False, True])
+def test_autograd_sees_the_step(slow):
+    """A graph that saved a parameter cannot be run backward over its new values; nor one that saved a clipped
+    gradient."""
+    params = _params([300], torch.float32)
+    opt = AdamW(params, **HP)
+    _grads(params, 1)
+    opt.step()
+    loss = (params[0] * params[0]).sum()
+    if slow:
+        opt._slow_step(opt._ready(), None)
+    else:
+        opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    before = params[0].grad._version
+    grad_norm(params)
+    assert params[0].grad._version == before
+    clip_grad_norm_(params, 1.0)
+    assert params[0].grad._version > before
 
 
 def test_grad_scaler_and_closure():
