@@ -244,7 +244,8 @@ typedef struct smo_adamw_hyper {
  * c = rint(top * sqrt(|x| * (1 / s))) with x's sign, top = 127 or 255; a
  * positive u is never stored as 0.  A block that holds a NaN gets the scale
  * NaN.  m_q, v_q: nb * q_block bytes, 16-byte aligned; the codes behind n are
- * written as 0.  The update uses m and u before they are coded. */
+ * written as 0.  The update uses m and u before they are coded; its quotient
+ * (which decides no code) may be off by a few units in the last place. */
 typedef struct smo_adamw_tensor {
     void *param;
     const void *grad;

@@ -143,7 +143,9 @@ class _AdamWBase(Optimizer):
         # norm of the gradients that the last step saw, before clipping; kept
         # only with max_grad_norm, and overwritten by the next step
         self.last_grad_norm = None
-        self._plan = None       # (capsule of the C++ host path, device index, number of tensors)
+        # the C++ host path of what it was made of: (state, param groups, capsule,
+        # device index, number of tensors)
+        self._plan = None
         self._workspace = {}    # device index -> (workspace, norm)
         self._scalars = {}      # device index -> scalars of each tensor (capturable)
         self._kept = []         # outgrown ones of the two, which captured graphs may hold
@@ -313,7 +315,8 @@ class _AdamWBase(Optimizer):
         if grad_scale is not None:
             if not torch.is_tensor(grad_scale) or grad_scale.dtype != torch.float32 or grad_scale.numel() != 1:
                 raise TypeError("grad_scale must be an fp32 tensor of one element")
-        if self._plan is not None:
+        plan = self._plan
+        if plan is not None and plan[0] is self.state and plan[1] is self.param_groups:
             rc = self._run_plan(grad_scale)
             if rc >= 0:
                 return loss
@@ -323,9 +326,11 @@ class _AdamWBase(Optimizer):
             if not items:
                 self.last_grad_norm = None
                 return loss
-            self._plan = _host_ext().adamw_plan(self.param_groups, self.state, _lib.address("smo_adamw_step"),
-                                                _lib.address("smo_adamw_advance") if self.capturable else 0)
-            if self._plan is None or self._run_plan(grad_scale) < 0:
+            made = _host_ext().adamw_plan(self.param_groups, self.state, _lib.address("smo_adamw_step"),
+                                          _lib.address("smo_adamw_advance") if self.capturable else 0)
+            if made is not None:
+                self._plan = (self.state, self.param_groups, *made)
+            if made is None or self._run_plan(grad_scale) < 0:
                 self._plan = None
                 self._slow_step(items, grad_scale)
         return loss
@@ -368,7 +373,7 @@ class _AdamWBase(Optimizer):
         return kept.data_ptr()
 
     def _run_plan(self, grad_scale) -> int:
-        cap, index, tensors = self._plan
+        _, _, cap, index, tensors = self._plan
         scale = self._scale_address(grad_scale, index)
         rc = _host_ext().adamw_run(cap, self._scalar_address(index, tensors), scale, *self._norm_buffers(index, tensors))
         if rc > 0:
@@ -540,7 +545,6 @@ class AdamW8bit(_AdamWBase):
     def _eight_bit(self, p, group) -> bool:
         return bool(group.get("compress", True)) and p.numel() >= max(1, self.min_8bit_numel)
 
-    @torch.no_grad()
     def moments(self, params=None, out=None):
         """``[(exp_avg, exp_avg_sq)]`` of ``params`` (default: every parameter
         that has a state) as fp32 tensors of the parameters' shapes: what the
@@ -550,14 +554,21 @@ class AdamW8bit(_AdamWBase):
         if params is None:
             params = [p for g in self.param_groups for p in g["params"] if self.state.get(p)]
         params = [params] if torch.is_tensor(params) else list(params)
-        if out is not None:
-            out = list(out)
-            got = _host_ext().adamw_moments(self.state, params, out, _lib.address("smo_adamw_decode"))
-            if got >= 0:
-                _lib.check(got, "smo_adamw_decode")
-                return out
-            if len(out) != len(params):
-                raise ValueError(f"{len(params)} parameters, {len(out)} outputs")
+        if out is None:
+            return self._moments(params)
+        out = list(out)
+        got = _host_ext().adamw_moments(self.state, params, out, _lib.address("smo_adamw_decode"))
+        if got < 0:
+            return self._moments(params, out)
+        if got > 0:
+            _lib.check(got, "smo_adamw_decode")
+        return out
+
+    @torch.no_grad()
+    def _moments(self, params, out=None):
+        """Refusals, parameters with fp32 moments among the others, several devices."""
+        if out is not None and len(out) != len(params):
+            raise ValueError(f"{len(params)} parameters, {len(out)} outputs")
         for p in params:
             if not self.state.get(p):
                 raise KeyError("moments of a parameter that has no state yet")

@@ -354,6 +354,15 @@ def test_plan_follows_replaced_tensors():
     params.append(extra[0])
     refs.append(Plain32(_np(extra[0])))
     both(3e-3)
+    opt.param_groups = [dict(g) for g in opt.param_groups]
+    opt.param_groups[0]["lr"] = opt.param_groups[1]["lr"] = 2e-3
+    both(2e-3)
+    state = type(opt.state)(dict)
+    for p, st in opt.state.items():
+        state[p] = {k: (t.clone() if torch.is_tensor(t) else t) for k, t in st.items()}
+    old, opt.state = opt.state, state
+    both(2e-3)
+    assert old[params[0]]["step"] + 1 == state[params[0]]["step"]
     for p, r in zip(params, refs):
         _check_param(_np(p), r, p.numel())
 
