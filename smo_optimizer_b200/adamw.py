@@ -557,7 +557,9 @@ class AdamW8bit(_AdamWBase):
         if out is None:
             return self._moments(params)
         out = list(out)
-        got = _host_ext().adamw_moments(self.state, params, out, _lib.address("smo_adamw_decode"))
+        plan = self._plan
+        plan = plan[2] if plan is not None and plan[0] is self.state else None
+        got = _host_ext().adamw_moments(self.state, params, out, _lib.address("smo_adamw_decode"), plan)
         if got < 0:
             return self._moments(params, out)
         if got > 0:

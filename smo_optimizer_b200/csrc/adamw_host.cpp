@@ -15,7 +15,7 @@
 #include <climits>
 #include <cmath>
 #include <cstring>
-#include <new>
+#include <unordered_map>
 #include <vector>
 
 #include <ATen/ops/empty.h>
@@ -72,6 +72,7 @@ struct AdamPlan {
     std::vector<smo_adamw_tensor> table;
     std::vector<smo_adamw_schedule> schedule;
     std::vector<const float *> lr_dev;    // per group
+    std::unordered_map<PyObject *, int> coded;  // entries with 8-bit moments, by parameter
     std::vector<long long> next_step;
     std::vector<double> hp_in;
 
@@ -204,6 +205,15 @@ bool fill_entry(AdamEntry &e, const at::Tensor &p, const at::Tensor &g) {
     return true;
 }
 
+// the state still holds the tensors that the entry's descriptor points into
+bool held_unchanged(const AdamEntry &e) {
+    for (int q = 0; q < e.nkeys; q++)
+        if (PyDict_GetItemWithError(e.state, e.keys[q]) != e.held[q] ||
+            THPVariable_Unpack(e.held[q]).data_ptr() != e.held_ptr[q])
+            return false;
+    return true;
+}
+
 bool read_step(PyObject *state, long long *out) {
     PyObject *st = PyDict_GetItemWithError(state, s_step);
     if (!st || !PyLong_CheckExact(st)) return false;
@@ -294,6 +304,7 @@ PyObject *build_plan(PyObject *groups_list, PyObject *state_map, unsigned long l
                 return none();
             }
             if (!fill_entry(e, p, g)) return none();
+            if (e.row.kind == SMO_ADAMW_8BIT) pl->coded.emplace(param, (int)pl->entries.size() - 1);
             pl->rows++;
         }
     }
@@ -342,10 +353,7 @@ int run_plan(AdamPlan &pl, const float *scale, float max_norm, float *norm_out, 
         if (dtype_code(p.scalar_type()) != e.row.dtype || p.device().index() != pl.device) return -1;
         if (p.sizes() != c10::IntArrayRef(e.sizes) || p.strides() != c10::IntArrayRef(e.strides)) return -1;
         if (g.scalar_type() != p.scalar_type() || !same_layout(p, g)) return -1;
-        for (int q = 0; q < e.nkeys; q++)
-            if (PyDict_GetItemWithError(e.state, e.keys[q]) != e.held[q] ||
-                THPVariable_Unpack(e.held[q]).data_ptr() != e.held_ptr[q])
-                return -1;
+        if (!held_unchanged(e)) return -1;
         // a moment or a master copy that came or went makes another kind of entry
         if (PyDict_GET_SIZE(e.state) != e.nstate) return -1;
         smo_adamw_tensor &r = pl.table[m];
@@ -459,13 +467,21 @@ PyObject *adamw_hyper_bytes(PyObject *, PyObject *args) {
     return PyBytes_FromStringAndSize((const char *)&h, sizeof(h));
 }
 
-// adamw_moments(state_mapping, [param], [(exp_avg, exp_avg_sq)], decode_fn_addr):
-// 0, an smo_status, or -1 where a parameter or an output is not as it has to be
+// adamw_moments(state_mapping, [param], [(exp_avg, exp_avg_sq)], decode_fn_addr, plan capsule or None):
+// 0, an smo_status, or -1 where a parameter or an output is not as it has to be.  The plan, made of the same
+// mapping, saves looking for and checking the states of its parameters.
 PyObject *adamw_moments(PyObject *, PyObject *args) {
-    PyObject *state_map, *params, *outs;
+    PyObject *state_map, *params, *outs, *cap;
     unsigned long long fn;
-    if (!PyArg_ParseTuple(args, "O!O!O!K", &PyDict_Type, &state_map, &PyList_Type, &params, &PyList_Type, &outs, &fn))
+    if (!PyArg_ParseTuple(args, "O!O!O!KO", &PyDict_Type, &state_map, &PyList_Type, &params, &PyList_Type, &outs, &fn,
+                          &cap))
         return nullptr;
+    const AdamPlan *pl = nullptr;
+    if (cap != Py_None) {
+        pl = (AdamPlan *)PyCapsule_GetPointer(cap, "smo_adamw_plan");
+        if (!pl) return nullptr;
+        if (pl->generation != g_state_generation) pl = nullptr;
+    }
     try {
         const Py_ssize_t n = PyList_GET_SIZE(params);
         if (PyList_GET_SIZE(outs) != n) return PyLong_FromLong(-1);
@@ -474,21 +490,39 @@ PyObject *adamw_moments(PyObject *, PyObject *args) {
         PyObject *const keys[4] = {s_m_q, s_m_s, s_v_q, s_v_s};
         for (Py_ssize_t i = 0; i < n; i++) {
             PyObject *param = PyList_GET_ITEM(params, i), *pair = PyList_GET_ITEM(outs, i), *t[4];
-            PyObject *state = THPVariable_Check(param) ? PyDict_GetItemWithError(state_map, param) : nullptr;
-            bool ok = state && PyDict_Check(state) && PyTuple_Check(pair) && PyTuple_GET_SIZE(pair) == 2 &&
+            bool ok = THPVariable_Check(param) && PyTuple_Check(pair) && PyTuple_GET_SIZE(pair) == 2 &&
                       THPVariable_Check(PyTuple_GET_ITEM(pair, 0)) && THPVariable_Check(PyTuple_GET_ITEM(pair, 1));
-            for (int k = 0; ok && k < 4; k++) {
-                t[k] = state_tensor(state, keys[k]);
-                ok = t[k] != nullptr;
-            }
             smo_adamw_tensor &r = table[(size_t)i];
             std::memset(&r, 0, sizeof(r));
             if (ok) {
                 const at::Tensor &p = THPVariable_Unpack(param);
-                ok = p.is_cuda() && (device < 0 || p.device().index() == device);
+                const auto known = pl ? pl->coded.find(param) : std::unordered_map<PyObject *, int>::const_iterator();
+                const AdamEntry *e = pl && known != pl->coded.end() ? &pl->entries[(size_t)known->second] : nullptr;
+                if (e && (!held_unchanged(*e) || p.numel() != e->row.n || p.device().index() != pl->device)) e = nullptr;
+                if (e) {
+                    r.m_q = e->row.m_q;
+                    r.m_s = e->row.m_s;
+                    r.v_q = e->row.v_q;
+                    r.v_s = e->row.v_s;
+                    r.q_block = e->row.q_block;
+                } else {
+                    PyObject *state = PyDict_GetItemWithError(state_map, param);
+                    ok = p.is_cuda() && state && PyDict_Check(state);
+                    for (int k = 0; ok && k < 4; k++) {
+                        t[k] = state_tensor(state, keys[k]);
+                        ok = t[k] != nullptr;
+                    }
+                    r.q_block = ok ? codes_block(t, p) : 0;
+                    ok = ok && r.q_block;
+                    if (ok) {
+                        r.m_q = (int8_t *)THPVariable_Unpack(t[0]).data_ptr();
+                        r.m_s = (float *)THPVariable_Unpack(t[1]).data_ptr();
+                        r.v_q = (uint8_t *)THPVariable_Unpack(t[2]).data_ptr();
+                        r.v_s = (float *)THPVariable_Unpack(t[3]).data_ptr();
+                    }
+                }
+                ok = ok && (device < 0 || p.device().index() == device);
                 if (ok) device = p.device().index();
-                r.q_block = ok ? codes_block(t, p) : 0;
-                ok = ok && r.q_block;
                 for (int k = 0; ok && k < 2; k++) {
                     const at::Tensor &o = THPVariable_Unpack(PyTuple_GET_ITEM(pair, k));
                     ok = o.scalar_type() == c10::ScalarType::Float && o.device() == p.device() &&
@@ -496,16 +530,12 @@ PyObject *adamw_moments(PyObject *, PyObject *args) {
                     (k ? r.exp_avg_sq : r.exp_avg) = ok ? (float *)o.data_ptr() : nullptr;
                 }
                 r.n = p.numel();
+                r.kind = SMO_ADAMW_8BIT;
             }
             if (!ok) {
                 PyErr_Clear();
                 return PyLong_FromLong(-1);
             }
-            r.kind = SMO_ADAMW_8BIT;
-            r.m_q = (int8_t *)THPVariable_Unpack(t[0]).data_ptr();
-            r.m_s = (float *)THPVariable_Unpack(t[1]).data_ptr();
-            r.v_q = (uint8_t *)THPVariable_Unpack(t[2]).data_ptr();
-            r.v_s = (float *)THPVariable_Unpack(t[3]).data_ptr();
         }
         if (n == 0) return PyLong_FromLong(0);
         c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
