@@ -148,7 +148,7 @@ class _AdamWBase(Optimizer):
         self._plan = None
         self._workspace = {}    # device index -> (workspace, norm)
         self._scalars = {}      # device index -> scalars of each tensor (capturable)
-        self._kept = []         # outgrown ones of the two, which captured graphs may hold
+        self._kept = []         # outgrown and replaced ones of the two, which captured graphs may hold
 
     # ---------------------------------------------------------------- state
 
@@ -161,8 +161,10 @@ class _AdamWBase(Optimizer):
     def __setstate__(self, state):
         super().__setstate__(state)
         self._plan = None
-        self._workspace, self._scalars = {}, {}
         self._kept = getattr(self, "_kept", [])
+        for held in ("_workspace", "_scalars"):
+            self._kept += getattr(self, held, {}).values()
+            setattr(self, held, {})
         self.last_grad_norm = None
 
     def add_param_group(self, param_group):
@@ -233,7 +235,7 @@ class _AdamWBase(Optimizer):
         """Loads what ``state_dict()`` of this class, of the other one here or of
         ``torch.optim.AdamW`` returned: moments are kept in 32 bits, and brought
         into 8 bits or out of them (or to another block size) where this
-        optimizer holds them so."""
+        optimizer holds them so.  The loaded tensors are copied."""
         last = {}
         # registered last: sees the dict as the other hooks leave it
         hook = self.register_load_state_dict_pre_hook(lambda opt, sd: last.update(sd))
@@ -251,10 +253,11 @@ class _AdamWBase(Optimizer):
             if not saved:
                 continue
             # torch's loader has cast every tensor to the parameter's type: take the saved ones
-            state = {"step": self._step_value(p, saved.get("step", 0))}
+            step = saved.get("step", 0)
+            state = {"step": self._step_value(p, step.clone() if torch.is_tensor(step) else step)}
             for key, dtype in _STATE_DTYPES.items():
                 if torch.is_tensor(saved.get(key)):
-                    state[key] = saved[key].to(device=p.device, dtype=dtype)
+                    state[key] = saved[key].to(device=p.device, dtype=dtype, copy=True)
             if not self.master_weights or p.dtype == torch.float32:
                 state.pop("master", None)
             self.state[p] = self._adopt(p, state, group)

@@ -498,6 +498,26 @@ def test_state_dict_continues_with_the_same_bits(cls):
         assert torch.equal(a.state[p]["master"], b.state[q]["master"])
 
 
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("cls", [AdamW, AdamW8bit])
+def test_loaded_states_share_nothing(cls, capturable):
+    pa, pb = _params([5000, 30], torch.bfloat16), _params([5000, 30], torch.bfloat16)
+    kw = dict(HP, master_weights=True, capturable=capturable, max_grad_norm=0.5)
+    a, b = cls(pa, **kw), cls(pb, **kw)
+    _grads(pa, 1)
+    a.step()
+    b.load_state_dict(a.state_dict())
+    kept = copy.deepcopy(a.state_dict())
+    for step in range(2):
+        _grads(pb, 2 + step)
+        b.step()
+    for p, (i, st) in zip(pa, kept["state"].items()):
+        for k, t in st.items():
+            now = a.state[p][k]
+            assert torch.equal(now, t) if torch.is_tensor(t) else now == t, k
+    assert float(b.state[pb[0]]["step"]) == 3
+
+
 def test_loads_a_torch_adamw_state():
     params = _params([5000, 30], torch.float32)
     ref = torch.optim.AdamW(params, **HP)
