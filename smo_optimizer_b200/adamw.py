@@ -51,7 +51,7 @@ def _norm(parameters, max_norm, what):
     if got is None:
         got = _norm_of_copies(parameters, max_norm, what, ext, fn, ws)
         if got is None:
-            return torch.zeros(())
+            return torch.zeros((), dtype=torch.float32, device="cpu")
     if got[0]:
         _lib.check(got[0], what)
     return got[1]
@@ -181,7 +181,7 @@ class _AdamWBase(Optimizer):
 
     def _init_state(self, p, group):
         state = self.state[p]
-        state["step"] = torch.zeros((), device=p.device) if self.capturable else 0
+        state["step"] = torch.zeros((), dtype=torch.float32, device=p.device) if self.capturable else 0
         if self._eight_bit(p, group):
             block = group["block_size"]
             nb = _host.num_blocks(p.numel(), block)
@@ -229,7 +229,7 @@ class _AdamWBase(Optimizer):
             if step.dtype == torch.float32 and step.device == p.device and step.numel() == 1:
                 return step
             return step.to(dtype=torch.float32, device=p.device).reshape(())
-        return torch.full((), float(step), device=p.device)
+        return torch.full((), float(step), dtype=torch.float32, device=p.device)
 
     def load_state_dict(self, state_dict):
         """Loads what ``state_dict()`` of this class, of the other one here or of
@@ -358,7 +358,7 @@ class _AdamWBase(Optimizer):
             if kept is not None:
                 self._kept.append(kept)
             dev = torch.device("cuda", index)
-            kept = (torch.empty(need, dtype=torch.uint8, device=dev), torch.zeros((), device=dev))
+            kept = (torch.empty(need, dtype=torch.uint8, device=dev), torch.zeros((), dtype=torch.float32, device=dev))
             self._workspace[index] = kept
         self.last_grad_norm = kept[1]
         return float(self.max_grad_norm), kept[1].data_ptr(), kept[0].data_ptr(), kept[0].numel()
@@ -371,7 +371,8 @@ class _AdamWBase(Optimizer):
         if kept is None or kept.shape[0] < tensors:
             if kept is not None:
                 self._kept.append(kept)
-            kept = torch.empty((tensors, len(_lib.ADAMW_HYPER_DTYPE)), device=torch.device("cuda", index))
+            kept = torch.empty((tensors, len(_lib.ADAMW_HYPER_DTYPE)), dtype=torch.float32,
+                               device=torch.device("cuda", index))
             self._scalars[index] = kept
         return kept.data_ptr()
 
