@@ -441,11 +441,10 @@ class _AdamWBase(Optimizer):
         coded = all(k in state for k in _CODE_KEYS)
         floats = ("master",) if "master" in state else ()
         floats += () if coded else _FLOAT_KEYS
-        for key in floats + (_CODE_KEYS if coded else ()):
+        for key in floats:
             t = state.get(key)
-            if not torch.is_tensor(t) or t.dtype != _STATE_DTYPES[key] or t.device != p.device:
-                raise TypeError(f"state['{key}'] must be a {_STATE_DTYPES[key]} tensor on {p.device}")
-            if key in floats and t.shape != p.shape:
+            _check_state_tensor(p, key, t)
+            if t.shape != p.shape:
                 raise ValueError(f"state['{key}'] must have the parameter's shape {tuple(p.shape)}")
         held = {k: state[k] for k in floats}
         direct = _same_dense_layout(p, *held.values()) and (not coded or p.is_contiguous())
@@ -472,14 +471,7 @@ class _AdamWBase(Optimizer):
             rec[k] = local(t, True).data_ptr()
         rec["n"], rec["dtype"] = p.numel(), _DTYPE_CODES[p.dtype]
         if coded:
-            block = state["m_q"].shape[-1]
-            nb = _host.num_blocks(p.numel(), block) if block in BLOCK_SIZES else -1
-            for k in _CODE_KEYS:
-                t = state[k]
-                if t.numel() != (nb * block if k.endswith("_q") else nb) or not t.is_contiguous():
-                    raise ValueError(f"state['{k}'] must be contiguous, with a block size of {BLOCK_SIZES}")
-                rec[k] = t.data_ptr()
-            rec["kind"], rec["q_block"] = _lib.SMO_ADAMW_8BIT, block
+            _coded_row(rec, p, state)
         else:
             rec["kind"] = _lib.SMO_ADAMW_F32
         if not self.capturable:
@@ -596,11 +588,22 @@ class AdamW8bit(_AdamWBase):
         return out
 
 
+def _check_state_tensor(p, key, t):
+    if not torch.is_tensor(t) or t.dtype != _STATE_DTYPES[key] or t.device != p.device:
+        raise TypeError(f"state['{key}'] must be a {_STATE_DTYPES[key]} tensor on {p.device}")
+
+
 def _coded_row(rec, p, state):
-    block = state["m_q"].shape[1]
-    rec["kind"], rec["q_block"], rec["n"] = _lib.SMO_ADAMW_8BIT, block, p.numel()
     for k in _CODE_KEYS:
-        rec[k] = state[k].data_ptr()
+        _check_state_tensor(p, k, state.get(k))
+    block = state["m_q"].shape[-1] if state["m_q"].dim() else 0
+    nb = _host.num_blocks(p.numel(), block) if block in BLOCK_SIZES else -1
+    for k in _CODE_KEYS:
+        t = state[k]
+        if t.numel() != (nb * block if k.endswith("_q") else nb) or not t.is_contiguous():
+            raise ValueError(f"state['{k}'] must be contiguous, with a block size of {BLOCK_SIZES}")
+        rec[k] = t.data_ptr()
+    rec["kind"], rec["q_block"], rec["n"] = _lib.SMO_ADAMW_8BIT, block, p.numel()
 
 
 def _launch_codes(name, rows):
