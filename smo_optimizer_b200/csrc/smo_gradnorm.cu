@@ -183,7 +183,7 @@ int run_type(GradOf grad_of, const void *items, int32_t n, int32_t dtype, double
         }
         if (end) break;
         b.d[b.n] = GradDesc{g.grad, g.n};
-        b.start[b.n + 1] = b.start[b.n] + (int32_t)((g.n + kChunk - 1) / kChunk);
+        b.start[b.n + 1] = b.start[b.n] + (int32_t)chunks_of(g.n, kChunk);
         b.n++;
     }
     return SMO_OK;
@@ -218,7 +218,7 @@ static int validate_grads(const smo_grad *g, int32_t n) {
         if (g[i].n == 0) continue;
         if (!g[i].grad) return SMO_ERR_INVALID;
         if (!is_aligned(g[i].grad, dtype_bytes(g[i].dtype))) return SMO_ERR_ALIGNMENT;
-        chunks += (g[i].n + kChunk - 1) / kChunk;
+        chunks += chunks_of(g[i].n, kChunk);
         if (chunks > INT32_MAX) return SMO_ERR_INVALID;  // they are counted in 32 bits (1.7e13 elements)
     }
     return SMO_OK;

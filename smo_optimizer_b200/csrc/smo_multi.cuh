@@ -95,6 +95,8 @@ inline int cuda_status(cudaError_t e) {
     return SMO_ERR_CUDA;
 }
 
+// chunks of n >= 0 elements
+inline int64_t chunks_of(int64_t n, int64_t chunk) { return n / chunk + (n % chunk != 0); }
 inline bool is_aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
 inline size_t dtype_bytes(int32_t dtype) { return dtype == SMO_DTYPE_F32 ? 4 : 2; }
 inline bool known_dtype(int32_t dtype) {
