@@ -36,6 +36,15 @@ _STATE_DTYPES = {"exp_avg": torch.float32, "exp_avg_sq": torch.float32, "master"
                  "m_s": torch.float32, "v_q": torch.uint8, "v_s": torch.float32}
 
 
+def _check_options(name, group, defaults):
+    """Refuses options of torch's AdamW and Adam under which the step would be another one."""
+    for key in ("maximize", "amsgrad"):
+        if group.get(key):
+            raise ValueError(f"{name} has no {key}")
+    if not group.get("decoupled_weight_decay", True) and group.get("weight_decay", defaults["weight_decay"]):
+        raise ValueError(f"{name} decays the weights themselves: decoupled_weight_decay=False is another step")
+
+
 def _stream(dev) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
 
@@ -168,6 +177,8 @@ class _AdamWBase(Optimizer):
         self.last_grad_norm = None
 
     def add_param_group(self, param_group):
+        if isinstance(param_group, dict):
+            _check_options(self._name, param_group, self.defaults)
         super().add_param_group(param_group)
         # torch only warns of a parameter that a group holds twice; stepped in one
         # launch, the two would write the same memory
@@ -235,10 +246,17 @@ class _AdamWBase(Optimizer):
         """Loads what ``state_dict()`` of this class, of the other one here or of
         ``torch.optim.AdamW`` returned: moments are kept in 32 bits, and brought
         into 8 bits or out of them (or to another block size) where this
-        optimizer holds them so.  The loaded tensors are copied."""
+        optimizer holds them so.  The loaded tensors are copied.  Groups with
+        ``maximize``, ``amsgrad`` or a decay that is not decoupled are refused."""
         last = {}
+
+        def check(opt, sd):
+            for group in sd["param_groups"]:
+                _check_options(self._name, group, self.defaults)
+            last.update(sd)
+
         # registered last: sees the dict as the other hooks leave it
-        hook = self.register_load_state_dict_pre_hook(lambda opt, sd: last.update(sd))
+        hook = self.register_load_state_dict_pre_hook(check)
         try:
             super().load_state_dict(state_dict)
         finally:
