@@ -175,6 +175,8 @@ class _AdamWBase(Optimizer):
             self._kept += getattr(self, held, {}).values()
             setattr(self, held, {})
         self.last_grad_norm = None
+        for p, held in self.__dict__.pop("_incoming", ()):
+            self.state[p] = held
 
     def add_param_group(self, param_group):
         if isinstance(param_group, dict):
@@ -247,38 +249,43 @@ class _AdamWBase(Optimizer):
         ``torch.optim.AdamW`` returned: moments are kept in 32 bits, and brought
         into 8 bits or out of them (or to another block size) where this
         optimizer holds them so.  The loaded tensors are copied.  Groups with
-        ``maximize``, ``amsgrad`` or a decay that is not decoupled are refused."""
-        last = {}
-
-        def check(opt, sd):
-            for group in sd["param_groups"]:
+        ``maximize``, ``amsgrad`` or a decay that is not decoupled are refused; a
+        load that is refused leaves the optimizer as it was."""
+        def prepare(opt, sd):
+            groups = [{**self.defaults, **g} for g in sd["param_groups"]]
+            for group in groups:
                 _check_options(self._name, group, self.defaults)
-            last.update(sd)
+            if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+                return None  # torch refuses it
+            own = chain.from_iterable(g["params"] for g in self.param_groups)
+            names = [(name, g) for g in groups for name in g["params"]]
+            self._incoming = [(p, self._loaded(p, sd["state"][name], group)) for p, (name, group) in zip(own, names)
+                              if sd["state"].get(name)]
+            # torch's loader would cast every tensor to the parameter's type
+            taken = {name for name, _ in names}
+            return dict(sd, state={k: v for k, v in sd["state"].items() if k not in taken})
 
         # registered last: sees the dict as the other hooks leave it
-        hook = self.register_load_state_dict_pre_hook(check)
+        hook = self.register_load_state_dict_pre_hook(prepare)
         try:
-            super().load_state_dict(state_dict)
+            super().load_state_dict(state_dict)  # its __setstate__() takes what comes in
         finally:
             hook.remove()
+            self._incoming = ()
         for group in self.param_groups:
             for key, value in self.defaults.items():
                 group.setdefault(key, value)
-        names = chain.from_iterable(g["params"] for g in last["param_groups"])
-        own = ((p, g) for g in self.param_groups for p in g["params"])
-        for name, (p, group) in zip(names, own):
-            saved = last["state"].get(name)
-            if not saved:
-                continue
-            # torch's loader has cast every tensor to the parameter's type: take the saved ones
-            step = saved.get("step", 0)
-            state = {"step": self._step_value(p, step.clone() if torch.is_tensor(step) else step)}
-            for key, dtype in _STATE_DTYPES.items():
-                if torch.is_tensor(saved.get(key)):
-                    state[key] = saved[key].to(device=p.device, dtype=dtype, copy=True)
-            if not self.master_weights or p.dtype == torch.float32:
-                state.pop("master", None)
-            self.state[p] = self._adopt(p, state, group)
+
+    def _loaded(self, p, saved, group):
+        """A saved state as this optimizer holds it, in tensors of its own."""
+        step = saved.get("step", 0)
+        state = {"step": self._step_value(p, step.clone() if torch.is_tensor(step) else step)}
+        for key, dtype in _STATE_DTYPES.items():
+            if torch.is_tensor(saved.get(key)):
+                state[key] = saved[key].to(device=p.device, dtype=dtype, copy=True)
+        if not self.master_weights or p.dtype == torch.float32:
+            state.pop("master", None)
+        return self._adopt(p, state, group)
 
     def _adopt(self, p, state, group):
         """A loaded state as this optimizer holds it."""

@@ -65,3 +65,93 @@ def test_options_that_leave_the_step_as_it_is(cls):
     group = opt.param_groups[0]
     assert group["lr"] == 1e-2 and not group["maximize"] and not group["amsgrad"]
     assert set(opt.state[group["params"][0]]) == {"step", "exp_avg", "exp_avg_sq"}
+
+
+def _coded(n, block):
+    nb = -(-n // block)
+    r = torch.Generator().manual_seed(n)
+    return {"step": 3, "m_q": torch.randint(-127, 128, (nb, block), generator=r).to(torch.int8),
+            "v_q": torch.randint(0, 256, (nb, block), generator=r).to(torch.uint8),
+            "m_s": torch.rand((nb, 1), generator=r), "v_s": torch.rand((nb, 1), generator=r)}
+
+
+def _floats(n, seed=0):
+    r = torch.Generator().manual_seed(seed)
+    return {"step": 2, "exp_avg": torch.randn(n, generator=r), "exp_avg_sq": torch.rand(n, generator=r)}
+
+
+def _loaded(cls, dtype=torch.bfloat16):
+    """An optimizer over three bf16 parameters with a loaded state each."""
+    sizes = [30, 5000, 257]
+    opt = cls([{"params": [_p(n, dtype) for n in sizes[:2]]}, {"params": [_p(sizes[2], dtype)], "lr": 0.5}], lr=0.25)
+    sd = opt.state_dict()
+    sd["state"] = {i: _floats(n, i) for i, n in enumerate(sizes)}
+    if cls is AdamW8bit:
+        sd["state"][1] = _coded(5000, 128)
+    opt.load_state_dict(sd)
+    return opt, copy.deepcopy(opt.state_dict())
+
+
+def _same_state(a, b):
+    assert a["param_groups"] == b["param_groups"] and a["state"].keys() == b["state"].keys()
+    for i in a["state"]:
+        assert a["state"][i].keys() == b["state"][i].keys()
+        for k, t in a["state"][i].items():
+            u = b["state"][i][k]
+            assert (t.dtype == u.dtype and torch.equal(t, u)) if torch.is_tensor(t) else t == u, (i, k)
+
+
+@BOTH
+@pytest.mark.parametrize("spoil", [
+    lambda sd: sd["state"][2].update(exp_avg=torch.zeros(256)), lambda sd: sd["state"][2].pop("exp_avg_sq"),
+    lambda sd: sd["state"][0].update(step="many"), lambda sd: sd["state"][2].update(master=torch.zeros(1, 257)),
+    lambda sd: sd["state"].update({1: dict(_coded(5000, 128), m_q=torch.zeros((39, 128), dtype=torch.int8))}),
+    lambda sd: sd["param_groups"].pop(), lambda sd: sd["param_groups"][0]["params"].pop(),
+    lambda sd: sd["param_groups"][1].update(maximize=True)])
+def test_a_refused_load_changes_nothing(cls, spoil):
+    opt, before = _loaded(cls)
+    opt.master_weights = True
+    held = [dict(opt.state[p]) for g in opt.param_groups for p in g["params"]]
+    sd = copy.deepcopy(before)
+    for g in sd["param_groups"]:
+        g["lr"] = 7.0
+    spoil(sd)
+    with pytest.raises(ValueError):
+        opt.load_state_dict(sd)
+    _same_state(opt.state_dict(), before)
+    now = [opt.state[p] for g in opt.param_groups for p in g["params"]]
+    assert all(a[k] is b[k] for a, b in zip(now, held) for k in b)
+    opt.load_state_dict(before)
+    _same_state(opt.state_dict(), before)
+
+
+@BOTH
+def test_load_hooks_see_and_shape_what_is_loaded(cls):
+    opt, before = _loaded(cls)
+    seen = []
+
+    def halve(o, sd):
+        sd = copy.deepcopy(sd)
+        sd["state"][0]["exp_avg"] *= 0.5
+        sd["state"]["note"] = "kept"
+        return sd
+
+    opt.register_load_state_dict_pre_hook(halve)
+    opt.register_load_state_dict_post_hook(lambda o: seen.append({k: v for k, v in o.state[o.param_groups[0]["params"][0]].items()}))
+    opt.load_state_dict(before)
+    p = opt.param_groups[0]["params"][0]
+    assert opt.state[p]["exp_avg"].dtype == torch.float32
+    assert torch.equal(opt.state[p]["exp_avg"], before["state"][0]["exp_avg"] * 0.5)
+    assert seen[0]["exp_avg"] is opt.state[p]["exp_avg"] and opt.state["note"] == "kept"
+    shared = before["state"][0]["exp_avg_sq"].data_ptr()
+    assert opt.state[p]["exp_avg_sq"].data_ptr() != shared
+
+
+@BOTH
+def test_groups_without_an_option_take_the_optimizers(cls):
+    opt, before = _loaded(cls)
+    sd = copy.deepcopy(before)
+    for key in ("eps", "block_size"):
+        sd["param_groups"][0].pop(key, None)
+    opt.load_state_dict(sd)
+    _same_state(opt.state_dict(), before)
