@@ -66,11 +66,22 @@ def _norm(parameters, max_norm, what):
     return got[1]
 
 
+def _once(t):
+    """Index of one of each of t's repeated elements, or None where they overlap in another way than by strides of 0."""
+    extent = 1
+    for stride, size in sorted(zip(t.stride(), t.shape)):
+        if stride and size > 1:
+            if stride < extent:
+                return None
+            extent += stride * (size - 1)
+    return tuple(slice(0, 1) if stride == 0 else slice(None) for stride in t.stride())
+
+
 @torch.no_grad()
 def _norm_of_copies(parameters, max_norm, what, ext, fn, ws):
     """Refusals, no gradients at all (None), parameters given twice (taken once),
     and gradients with gaps or repeated elements: those are taken as copies,
-    written back when clipped."""
+    written back when clipped (a repeated element once)."""
     grads = [p.grad for p in {id(p): p for p in parameters}.values() if p.grad is not None]
     for g in grads:
         if g.is_sparse:
@@ -83,6 +94,9 @@ def _norm_of_copies(parameters, max_norm, what, ext, fn, ws):
             raise RuntimeError(f"{what} takes the gradients of one device; got {grads[0].device} and {g.device}")
     if not grads:
         return None
+    once = [_once(g) for g in grads] if max_norm > 0 else []
+    if None in once:
+        raise RuntimeError(f"{what} cannot scale a gradient whose elements overlap")
     holders = []
     for g in grads:
         holder = torch.nn.Parameter(torch.empty_like(g, memory_format=torch.contiguous_format))
@@ -92,9 +106,9 @@ def _norm_of_copies(parameters, max_norm, what, ext, fn, ws):
     if got is None:
         raise RuntimeError(f"{what}: two parameters share one gradient")
     if max_norm > 0:
-        for g, h in zip(grads, holders):
+        for g, h, index in zip(grads, holders, once):
             if h.grad.data_ptr() != g.data_ptr():
-                g.copy_(h.grad)
+                g[index].copy_(h.grad[index])
     return got
 
 
