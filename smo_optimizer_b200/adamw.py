@@ -104,7 +104,7 @@ def _norm_of_copies(parameters, max_norm, what, ext, fn, ws):
         holders.append(holder)
     got = ext.grad_norm(holders, max_norm, fn, ws)
     if got is None:
-        raise RuntimeError(f"{what}: two parameters share one gradient")
+        raise RuntimeError(f"{what}: two parameters share one gradient or, to be scaled, a part of it")
     if max_norm > 0:
         for g, h, index in zip(grads, holders, once):
             if h.grad.data_ptr() != g.data_ptr():
@@ -127,7 +127,8 @@ def grad_norm(parameters) -> torch.Tensor:
 def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     """Multiplies the gradients of all ``parameters`` in place by
     ``min(1, max_norm / (norm + 1e-6))`` and returns ``norm``, their 2-norm before
-    (see ``grad_norm``).  A norm that is NaN makes every gradient NaN.
+    (see ``grad_norm``).  A norm that is NaN makes every gradient NaN.  Gradients
+    that share elements are refused.
 
     ``AdamW`` and ``AdamW8bit`` clip within the step (``max_grad_norm``), without
     writing the gradients; this is for ``SMO``, ``SMO8bit`` and any other user of

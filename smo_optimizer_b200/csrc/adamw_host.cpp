@@ -16,6 +16,7 @@
 #include <cmath>
 #include <cstring>
 #include <unordered_map>
+#include <utility>
 #include <vector>
 
 #include <ATen/ops/empty.h>
@@ -548,8 +549,8 @@ PyObject *adamw_moments(PyObject *, PyObject *args) {
 }
 
 // grad_norm([parameter], max_norm, norm_fn_addr, workspace_fn_addr) -> (status, norm tensor), or None where a
-// gradient is not on the first one's CUDA device, of a known type and one span of memory, is there twice, or there is
-// none
+// gradient is not on the first one's CUDA device, of a known type and one span of memory, is there twice, shares
+// elements with another that would both be scaled, or there is none
 PyObject *grad_norm(PyObject *, PyObject *args) {
     PyObject *list;
     float max_norm;
@@ -573,13 +574,17 @@ PyObject *grad_norm(PyObject *, PyObject *args) {
             table.push_back(smo_grad{g.data_ptr(), g.numel(), dt, 0});
         }
         if (device < 0) Py_RETURN_NONE;
-        // a parameter given twice would be counted, and scaled, twice
-        std::vector<uintptr_t> seen;
-        seen.reserve(table.size());
+        // a parameter given twice would be counted, and scaled, twice; an element in two gradients by two threads
+        std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+        spans.reserve(table.size());
         for (const smo_grad &g : table)
-            if (g.n) seen.push_back((uintptr_t)g.grad);
-        std::sort(seen.begin(), seen.end());
-        if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) Py_RETURN_NONE;
+            if (g.n)
+                spans.emplace_back((uintptr_t)g.grad,
+                                   (uintptr_t)g.grad + (uintptr_t)g.n * (g.dtype == SMO_DTYPE_F32 ? 4 : 2));
+        std::sort(spans.begin(), spans.end());
+        for (size_t i = 1; i < spans.size(); i++)
+            if (spans[i].first == spans[i - 1].first || (max_norm > 0.0f && spans[i].first < spans[i - 1].second))
+                Py_RETURN_NONE;
         c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
         const size_t bytes = ((WorkspaceFn)(uintptr_t)ws_fn)((int32_t)table.size());
         const auto on = at::TensorOptions().device(c10::Device(c10::kCUDA, (c10::DeviceIndex)device));

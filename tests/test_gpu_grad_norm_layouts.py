@@ -80,3 +80,19 @@ def test_a_view_with_a_gap_and_the_span_around_it():
     norm = clip_grad_norm_(params, 0.5)
     assert _close(norm, want)
     assert torch.equal(buffer, kept * (torch.tensor(0.5, device="cuda") / (norm + 1e-6)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_spans_that_share_elements_are_not_clipped(dtype):
+    buffer = _randn(1000, seed=6, dtype=dtype)
+    kept = buffer.clone()
+    for a, b in ((buffer[:600], buffer[599:]), (buffer, buffer[400:410]), (buffer[1:3], buffer[:2])):
+        params = [_holder(a), _holder(b)]
+        assert _close(grad_norm(params), _exact(params))
+        for order in (params, params[::-1]):
+            with pytest.raises(RuntimeError, match="share"):
+                clip_grad_norm_(order, 0.5)
+        assert torch.equal(buffer, kept)
+    # neighbours share nothing
+    norm = clip_grad_norm_([_holder(buffer[:600]), _holder(buffer[600:])], 0.5)
+    assert torch.equal(buffer, (kept.float() * (torch.tensor(0.5, device="cuda") / (norm + 1e-6))).to(dtype))
