@@ -30,6 +30,8 @@ __all__ = ["AdamW", "AdamW8bit", "clip_grad_norm_", "grad_norm"]
 
 BLOCK_SIZES = (64, 128, 256)
 
+_LEAST_NORM = 2.0 ** -149  # as fp32 numbers smaller bounds are 0, which stands for no bound
+
 _FLOAT_KEYS = ("exp_avg", "exp_avg_sq")
 _CODE_KEYS = ("m_q", "m_s", "v_q", "v_s")
 _STATE_DTYPES = {"exp_avg": torch.float32, "exp_avg_sq": torch.float32, "master": torch.float32, "m_q": torch.int8,
@@ -134,7 +136,7 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     writing the gradients; this is for ``SMO``, ``SMO8bit`` and any other user of
     the gradients."""
     max_norm = float(max_norm)
-    if not max_norm > 0.0:
+    if not max_norm >= _LEAST_NORM:
         raise ValueError(f"Invalid max_norm: {max_norm}")
     return _norm(parameters, max_norm, "clip_grad_norm_")
 
@@ -158,7 +160,7 @@ class _AdamWBase(Optimizer):
             raise ValueError(f"Invalid beta parameter at index 1: {betas[1]}")
         if not 0.0 <= weight_decay:
             raise ValueError(f"Invalid weight_decay value: {weight_decay}")
-        if max_grad_norm is not None and not max_grad_norm > 0.0:
+        if max_grad_norm is not None and not max_grad_norm >= _LEAST_NORM:
             raise ValueError(f"Invalid max_grad_norm: {max_grad_norm}")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, **extra))
         self.master_weights = bool(master_weights)
@@ -392,6 +394,8 @@ class _AdamWBase(Optimizer):
         if self.max_grad_norm is None:
             self.last_grad_norm = None
             return 0.0, 0, 0, 0
+        if not self.max_grad_norm >= _LEAST_NORM:
+            raise ValueError(f"Invalid max_grad_norm: {self.max_grad_norm}")
         need = _lib.load().smo_grad_norm_workspace_size(tensors)
         kept = self._workspace.get(index)
         if kept is None or kept[0].numel() < need:
