@@ -47,6 +47,11 @@ def _check_options(name, group, defaults):
         raise ValueError(f"{name} decays the weights themselves: decoupled_weight_decay=False is another step")
 
 
+def _check_writable(what, tensors):
+    if not torch.is_inference_mode_enabled() and any(t.is_inference() for t in tensors):
+        raise RuntimeError(f"{what} writes inference tensors in inference mode only")
+
+
 def _stream(dev) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
 
@@ -97,6 +102,8 @@ def _norm_of_copies(parameters, max_norm, what, ext, fn, ws):
     if not grads:
         return None
     once = [_once(g) for g in grads] if max_norm > 0 else []
+    if max_norm > 0:
+        _check_writable(what, grads)
     if None in once:
         raise RuntimeError(f"{what} cannot scale a gradient whose elements overlap")
     holders = []
@@ -238,6 +245,7 @@ class _AdamWBase(Optimizer):
                 if p.dtype not in _DTYPE_CODES or grad.dtype != p.dtype:
                     raise TypeError(f"{self._name} (B200 build) steps fp32, bf16 or fp16 parameters with "
                                     f"gradients of the same dtype; got {p.dtype} / {grad.dtype}")
+                _check_writable(self._name, (p,))
                 state = self.state[p]
                 master = self.master_weights and p.dtype != torch.float32 and "master" not in state
                 if ("step" not in state or master) and torch.cuda.is_current_stream_capturing():
@@ -621,6 +629,7 @@ class AdamW8bit(_AdamWBase):
                 pairs[i] = pair
             return pairs
         for p, pair in zip(params, out):
+            _check_writable("moments", pair)
             for t in pair:
                 if t.dtype != torch.float32 or t.device != p.device or t.shape != p.shape or not t.is_contiguous():
                     raise TypeError(f"out must be contiguous fp32 tensors of the parameters' shapes on {p.device}")

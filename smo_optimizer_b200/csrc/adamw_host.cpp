@@ -20,6 +20,7 @@
 #include <vector>
 
 #include <ATen/ops/empty.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -116,6 +117,9 @@ int32_t dtype_code(c10::ScalarType t) {
         default: return -1;
     }
 }
+
+// torch refuses to write such a tensor in place: the Python path says so before anything is written
+bool not_writable(const at::Tensor &t) { return t.is_inference() && !c10::InferenceMode::is_enabled(); }
 
 // element k of one's memory is element k of the other's (a size of 1 may have any stride)
 bool same_layout(const at::Tensor &a, const at::Tensor &b) {
@@ -350,7 +354,7 @@ int run_plan(AdamPlan &pl, const float *scale, float max_norm, float *norm_out, 
             if (g.defined()) return -1;
             continue;
         }
-        if (!g.defined() || p.data_ptr() != e.param_ptr) return -1;
+        if (!g.defined() || p.data_ptr() != e.param_ptr || not_writable(p)) return -1;
         if (dtype_code(p.scalar_type()) != e.row.dtype || p.device().index() != pl.device) return -1;
         if (p.sizes() != c10::IntArrayRef(e.sizes) || p.strides() != c10::IntArrayRef(e.strides)) return -1;
         if (g.scalar_type() != p.scalar_type() || !same_layout(p, g)) return -1;
@@ -526,7 +530,7 @@ PyObject *adamw_moments(PyObject *, PyObject *args) {
                 if (ok) device = p.device().index();
                 for (int k = 0; ok && k < 2; k++) {
                     const at::Tensor &o = THPVariable_Unpack(PyTuple_GET_ITEM(pair, k));
-                    ok = o.scalar_type() == c10::ScalarType::Float && o.device() == p.device() &&
+                    ok = !not_writable(o) && o.scalar_type() == c10::ScalarType::Float && o.device() == p.device() &&
                          o.layout() == c10::kStrided && o.sizes() == p.sizes() && o.is_contiguous();
                     (k ? r.exp_avg_sq : r.exp_avg) = ok ? (float *)o.data_ptr() : nullptr;
                 }
@@ -550,7 +554,7 @@ PyObject *adamw_moments(PyObject *, PyObject *args) {
 
 // grad_norm([parameter], max_norm, norm_fn_addr, workspace_fn_addr) -> (status, norm tensor), or None where a
 // gradient is not on the first one's CUDA device, of a known type and one span of memory, is there twice, shares
-// elements with another that would both be scaled, or there is none
+// elements with another that would both be scaled or must not be written, or there is none
 PyObject *grad_norm(PyObject *, PyObject *args) {
     PyObject *list;
     float max_norm;
@@ -569,6 +573,7 @@ PyObject *grad_norm(PyObject *, PyObject *args) {
             const int32_t dt = dtype_code(g.scalar_type());
             if (dt < 0 || !g.is_cuda() || g.layout() != c10::kStrided || !g.is_non_overlapping_and_dense())
                 Py_RETURN_NONE;
+            if (max_norm > 0.0f && not_writable(g)) Py_RETURN_NONE;
             if (device >= 0 && g.device().index() != device) Py_RETURN_NONE;
             device = g.device().index();
             table.push_back(smo_grad{g.data_ptr(), g.numel(), dt, 0});
