@@ -634,6 +634,7 @@ class AdamW8bit(_AdamWBase):
                 if t.dtype != torch.float32 or t.device != p.device or t.shape != p.shape or not t.is_contiguous():
                     raise TypeError(f"out must be contiguous fp32 tensors of the parameters' shapes on {p.device}")
         _decode([(params[i], self.state[params[i]]) for i in coded], [out[i] for i in coded])
+        torch.autograd.graph.increment_version([t for i in coded for t in out[i]])
         for pair, dst in zip(pairs, out):
             if pair is not None:
                 for d, s in zip(dst, pair):

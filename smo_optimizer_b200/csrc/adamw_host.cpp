@@ -545,7 +545,12 @@ PyObject *adamw_moments(PyObject *, PyObject *args) {
         if (n == 0) return PyLong_FromLong(0);
         c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
         cudaStream_t stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
-        return PyLong_FromLong(((AdamwDecodeFn)(uintptr_t)fn)(table.data(), (int32_t)n, (void *)stream));
+        const int rc = ((AdamwDecodeFn)(uintptr_t)fn)(table.data(), (int32_t)n, (void *)stream);
+        if (rc == SMO_OK)
+            for (Py_ssize_t i = 0; i < n; i++)
+                for (int k = 0; k < 2; k++)
+                    THPVariable_Unpack(PyTuple_GET_ITEM(PyList_GET_ITEM(outs, i), k)).unsafeGetTensorImpl()->bump_version();
+        return PyLong_FromLong(rc);
     } catch (const std::exception &e) {
         PyErr_SetString(PyExc_RuntimeError, e.what());
         return nullptr;

@@ -46,3 +46,19 @@ def test_inference_tensors_are_written_in_inference_mode_only(cls):
         if cls is AdamW8bit:
             assert opt.moments(params, out=out) is not None and out[0][1].any()
     assert all(opt.state[p]["step"] == 2 for p in params)
+
+
+@pytest.mark.parametrize("mixed", [False, True])
+def test_moments_written_to_tensors_of_the_caller(mixed):
+    """All parameters coded, and one with fp32 moments among them (another path)."""
+    params = _params([5000, 30] if mixed else [5000, 6000])
+    opt = AdamW8bit(params)
+    opt.step()
+    out = [tuple(torch.zeros_like(p) for _ in range(2)) for p in params]
+    w = torch.ones(params[0].shape, device="cuda", requires_grad=True)
+    loss = (w * out[0][1]).sum()  # keeps out[0][1] for the gradient of w
+    before = [t._version for pair in out for t in pair]
+    opt.moments(params, out=out)
+    assert all(t._version > v for t, v in zip((t for pair in out for t in pair), before))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
