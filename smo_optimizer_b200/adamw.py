@@ -564,9 +564,20 @@ class AdamW8bit(_AdamWBase):
     for ``s * sign(c) * (c / 127)**2`` and ``s * (c / 255)**2``, ``s`` the block's
     largest value: relative steps of 2 / c, so the larger values, which steer the
     update, are held most finely.  The update itself uses the moments before they
-    are coded.  Codes round to the nearest, so a moment that changes by less than
-    half its step between two updates keeps its code: as with other moments of
-    8 bits, a slow drift of a small second moment is followed late.
+    are coded.
+
+    Codes round to the nearest, so a moment that changes by less than half a code
+    in a step keeps its code, however many steps follow.  Without a gradient a
+    step shrinks codes by ``sqrt(beta1)`` and ``beta2 ** (1 / 4)``, or, in a block
+    without any gradient, the scale alone.  So beside an element that keeps the
+    block's scale up, m falls to 0.5 % of the block's largest and no further
+    (``beta1`` = 0.9), u to 2.3 % with ``beta2`` = 0.95, to 61 % with 0.99, and with
+    0.999 not at all; where m stays above 0 the parameter keeps moving.  With
+    gradients of a steady size u is right within 8 % (its median within 0.4 %) at
+    ``beta2`` of 0.99 and below; at 0.999 its median is 10 % too large after 3,000
+    steps, 16 % after 6,000 and 36 % after 12,000 (blocks of 128), and the updates
+    are that much too small.  Long runs want a ``beta2`` of 0.99 or less, or
+    ``AdamW``.
 
     Tensors of fewer than ``min_8bit_numel`` elements, and those of groups with
     ``compress=False``, keep fp32 moments as in ``AdamW``; ``protect_output``
