@@ -12,7 +12,7 @@ model their rounding.  The arithmetic is stated in include/smo_b200.h
 As with the other optimizers here the parameters are CUDA tensors (fp32, bf16
 or fp16) with gradients of their own type, the work runs on the current stream,
 and there is no CPU path.  All tensors of a step are written in one launch or in
-launches that overlap: they must not share memory.
+launches that overlap: parameters that share memory are refused.
 """
 
 from __future__ import annotations
@@ -149,6 +149,20 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------- optimizers
+
+
+def _check_apart(name, items):
+    """Refuses parameters that share elements, with each other (as far as each is one span of memory) or within."""
+    spans = []
+    for p, _, _, _ in items:
+        if p.is_contiguous():
+            if p.numel():
+                spans.append((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()))
+        elif _once(p) is None or any(stride == 0 and size > 1 for stride, size in zip(p.stride(), p.shape)):
+            raise ValueError(f"{name}: elements of a parameter share memory")
+    spans.sort()
+    if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+        raise ValueError(f"{name}: two parameters share memory")
 
 
 class _AdamWBase(Optimizer):
@@ -379,6 +393,7 @@ class _AdamWBase(Optimizer):
             if not items:
                 self.last_grad_norm = None
                 return loss
+            _check_apart(self._name, items)
             made = _host_ext().adamw_plan(self.param_groups, self.state, _lib.address("smo_adamw_step"),
                                           _lib.address("smo_adamw_advance") if self.capturable else 0)
             if made is not None:

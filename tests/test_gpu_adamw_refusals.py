@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from smo_optimizer_b200 import AdamW8bit
+from smo_optimizer_b200 import AdamW, AdamW8bit
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +42,27 @@ def test_moments_of_codes_that_do_not_fit(key, change, error):
     st[key] = kept
     assert all(torch.equal(a, b) for x, y in zip(opt.moments(params, out=out), want) for a, b in zip(x, y))
     assert st["step"] == 1
+
+
+@pytest.mark.parametrize("cls", [AdamW, AdamW8bit])
+def test_parameters_that_share_memory(cls):
+    params = _params([5000, 6000])
+    shared = torch.nn.Parameter(params[1].data[10:20])
+    shared.grad = torch.ones_like(shared)
+    opt = cls(params + [shared])
+    before = [p.detach().clone() for p in params]
+    for _ in range(2):
+        with pytest.raises(ValueError, match="share memory"):
+            opt.step()
+    assert all(torch.equal(p.detach(), q) for p, q in zip(params, before))
+    shared.grad = None
+    opt.step()
+    assert all(opt.state[p]["step"] == 1 for p in params)
+    shared.grad = torch.ones_like(shared)  # the plan of the last step does not hold it
+    with pytest.raises(ValueError, match="share memory"):
+        opt.step()
+    params[0].data = params[1].data[:5000]
+    shared.grad = None
+    with pytest.raises(ValueError, match="share memory"):
+        opt.step()
+    assert all(opt.state[p]["step"] == 1 for p in params)
