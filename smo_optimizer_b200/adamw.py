@@ -108,7 +108,8 @@ def _norm_of_copies(parameters, max_norm, what, ext, fn, ws):
         raise RuntimeError(f"{what} cannot scale a gradient whose elements overlap")
     holders = []
     for g in grads:
-        holder = torch.nn.Parameter(torch.empty_like(g, memory_format=torch.contiguous_format))
+        # only its gradient counts: a parameter of g's shape without that much memory
+        holder = torch.nn.Parameter(g.new_empty(()).expand(g.shape))
         holder.grad = g.contiguous()
         holders.append(holder)
     got = ext.grad_norm(holders, max_norm, fn, ws)

@@ -96,3 +96,15 @@ def test_spans_that_share_elements_are_not_clipped(dtype):
     # neighbours share nothing
     norm = clip_grad_norm_([_holder(buffer[:600]), _holder(buffer[600:])], 0.5)
     assert torch.equal(buffer, (kept.float() * (torch.tensor(0.5, device="cuda") / (norm + 1e-6))).to(dtype))
+
+
+@pytest.mark.parametrize("call", [grad_norm, lambda ps: clip_grad_norm_(ps, 0.5)], ids=["norm", "clip"])
+def test_copies_are_made_of_the_gradients_that_need_one_only(call):
+    big, gap = _holder(_randn(4_000_000, seed=7)), _holder(_randn(40, 33, seed=8)[:, :30])
+    call([big, gap])
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    norm = call([big, gap])
+    # the gradient is 16 MB; a workspace is a few times 4736 sums of 8 bytes
+    assert torch.cuda.max_memory_allocated() - before < 1 << 20, norm
