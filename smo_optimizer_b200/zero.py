@@ -79,7 +79,7 @@ def adamw_step_bytes(shape, eight_bit: bool, block: int = 128, min_8bit_numel: i
 
 
 def _step_cost(p, optimizer_cls, kwargs) -> int:
-    if issubclass(optimizer_cls, _AdamWBase):
+    if isinstance(optimizer_cls, type) and issubclass(optimizer_cls, _AdamWBase):
         return adamw_step_bytes(p.shape, issubclass(optimizer_cls, AdamW8bit), kwargs.get("block_size", 128),
                                 kwargs.get("min_8bit_numel", 4096), p.element_size(),
                                 kwargs.get("master_weights", False))
