@@ -245,7 +245,8 @@ typedef struct smo_adamw_hyper {
  * positive u is never stored as 0.  A block that holds a NaN gets the scale
  * NaN.  m_q, v_q: nb * q_block bytes, 16-byte aligned; the codes behind n are
  * written as 0.  The update uses m and u before they are coded; its quotient
- * (which decides no code) may be off by a few units in the last place. */
+ * (which decides no code) may be off by a few units in the last place, and takes
+ * subnormal denominators as 0: eps is 0 or at least 2^-126. */
 typedef struct smo_adamw_tensor {
     void *param;
     const void *grad;

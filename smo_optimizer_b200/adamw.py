@@ -39,12 +39,16 @@ _STATE_DTYPES = {"exp_avg": torch.float32, "exp_avg_sq": torch.float32, "master"
 
 
 def _check_options(name, group, defaults):
-    """Refuses options of torch's AdamW and Adam under which the step would be another one."""
+    """Refuses options of torch's AdamW and Adam under which the step would be another one, and values that it cannot
+    take."""
     for key in ("maximize", "amsgrad"):
         if group.get(key):
             raise ValueError(f"{name} has no {key}")
     if not group.get("decoupled_weight_decay", True) and group.get("weight_decay", defaults["weight_decay"]):
         raise ValueError(f"{name} decays the weights themselves: decoupled_weight_decay=False is another step")
+    # the 8-bit step's quotient takes smaller denominators as 0
+    if name == "AdamW8bit" and 0.0 < group.get("eps", defaults["eps"]) < 2.0 ** -126:
+        raise ValueError(f"Invalid epsilon value: {group.get('eps', defaults['eps'])} is below fp32's normal numbers")
 
 
 def _check_writable(what, tensors):

@@ -91,3 +91,14 @@ def test_codes_beside_a_live_element_keep_what_rounding_keeps():
             assert torch.equal(now[1], then[1])
             scale = float(opt.state[p][k + "_s"][1])
             assert abs(scale - whole ** steps) <= 1e-3 * whole ** steps, (k, scale)
+
+
+@pytest.mark.parametrize("eps", [2.0 ** -126, 1e-30])
+def test_the_least_eps_and_no_gradient(eps):
+    """Moments of 0 over eps alone: the parameter only decays."""
+    for cls in (AdamW, AdamW8bit):
+        p = torch.nn.Parameter(torch.ones(5000, device="cuda"))
+        p.grad = torch.zeros_like(p)
+        opt = cls([p], lr=0.5, eps=eps, weight_decay=0.5)
+        opt.step()
+        assert torch.equal(p.detach(), torch.full_like(p, 0.75))
