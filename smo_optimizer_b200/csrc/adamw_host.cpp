@@ -584,17 +584,23 @@ PyObject *grad_norm(PyObject *, PyObject *args) {
             table.push_back(smo_grad{g.data_ptr(), g.numel(), dt, 0});
         }
         if (device < 0) Py_RETURN_NONE;
-        // a parameter given twice would be counted, and scaled, twice; an element in two gradients by two threads
-        std::vector<std::pair<uintptr_t, uintptr_t>> spans;
-        spans.reserve(table.size());
-        for (const smo_grad &g : table)
-            if (g.n)
-                spans.emplace_back((uintptr_t)g.grad,
-                                   (uintptr_t)g.grad + (uintptr_t)g.n * (g.dtype == SMO_DTYPE_F32 ? 4 : 2));
-        std::sort(spans.begin(), spans.end());
-        for (size_t i = 1; i < spans.size(); i++)
-            if (spans[i].first == spans[i - 1].first || (max_norm > 0.0f && spans[i].first < spans[i - 1].second))
-                Py_RETURN_NONE;
+        // a gradient given twice (one address) would be counted twice, and an element that two gradients share
+        // scaled by two threads: runs of ascending spans first, mostly a few that are apart
+        const auto collide = [&](bool whole_runs) {
+            std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+            for (const smo_grad &g : table) {
+                if (!g.n) continue;
+                const uintptr_t a = (uintptr_t)g.grad, bytes = (uintptr_t)g.n * (g.dtype == SMO_DTYPE_F32 ? 4 : 2);
+                const uintptr_t end = max_norm > 0.0f ? a + bytes : a + 1;
+                if (whole_runs && !spans.empty() && a >= spans.back().second) spans.back().second = end;
+                else spans.emplace_back(a, end);
+            }
+            std::sort(spans.begin(), spans.end());
+            for (size_t i = 1; i < spans.size(); i++)
+                if (spans[i].first < spans[i - 1].second) return true;
+            return false;
+        };
+        if (collide(true) && collide(false)) Py_RETURN_NONE;
         c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
         const size_t bytes = ((WorkspaceFn)(uintptr_t)ws_fn)((int32_t)table.size());
         const auto on = at::TensorOptions().device(c10::Device(c10::kCUDA, (c10::DeviceIndex)device));
