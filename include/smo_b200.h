@@ -308,7 +308,8 @@ typedef struct smo_grad {
 
 /* The 2-norm over all elements of n tensors, written to norm_out (a device
  * float).  Products and sums are held in double and added in an order that
- * depends on the sizes alone, so the same gradients give the same bits.
+ * depends on the sizes and on the alignment of each tensor alone, so a call
+ * repeated gives the same bits.
  * max_norm > 0: the tensors are then multiplied in place by
  * min(1, max_norm / (norm + 1e-6)).  workspace: smo_grad_norm_workspace_size(n)
  * bytes, 256-byte aligned. */

@@ -131,8 +131,8 @@ def grad_norm(parameters) -> torch.Tensor:
     parameter) as one vector: an fp32 tensor of no dimensions on their device.
 
     Parameters without a gradient are left out.  Each gradient is read once;
-    squares and sums are held in double, in an order that depends on the sizes
-    alone, so the same gradients always give the same bits.  Nothing
+    squares and sums are held in double, in an order that depends on the sizes and
+    the addresses' alignment alone, so a call repeated gives the same bits.  Nothing
     synchronises.  A parameter given twice counts once.  Without any gradient:
     0, on the CPU."""
     return _norm(parameters, 0.0, "grad_norm")

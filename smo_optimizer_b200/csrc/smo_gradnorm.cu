@@ -1,11 +1,15 @@
 // smo_gradnorm.cu -- the 2-norm over many gradient tensors, and clipping by it.
 //
 // Each gradient is read once; squares and sums are held in double, so that the
-// norm is right to the last fp32 bit whatever the order of the additions (a
-// clipped step's 8-bit codes depend on every bit of the factor), and squares of
-// large elements do not overflow.  A CTA adds up every gridDim-th chunk and
-// writes one partial sum; a last CTA adds the partial sums in their order.  The
-// order goes by the sizes alone: no atomics, the same bits every time.
+// norm is right to the last fp32 bit (but where it lies within a 64-bit rounding of
+// the middle between two) whatever the order of the additions (a clipped step's
+// 8-bit codes depend on every bit of the factor), and squares of large elements do
+// not overflow.  A CTA adds up every gridDim-th chunk and writes one partial sum; a
+// last CTA, in a launch of its own, adds the partial sums in their order.  The order
+// goes only by the sizes and by which tensors are aligned: no atomics, the same bits
+// every time.  A tensor whose first element is not aligned is read element by
+// element throughout (38M bf16 elements in 148 tensors: 19.8 us aligned nowhere,
+// 16.4 us aligned; scaling included 48 and 30 us; fp32: 29.0 and 26.7, 72 and 70 us).
 #include <climits>
 #include <cstring>
 
