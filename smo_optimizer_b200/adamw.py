@@ -201,6 +201,7 @@ class _AdamWBase(Optimizer):
         self._workspace = {}    # device index -> (workspace, norm)
         self._scalars = {}      # device index -> scalars of each tensor (capturable)
         self._kept = []         # outgrown and replaced ones of the two, which captured graphs may hold
+        self._captured = False  # a step was captured: graphs hold the states' addresses
 
     # ---------------------------------------------------------------- state
 
@@ -214,12 +215,24 @@ class _AdamWBase(Optimizer):
         super().__setstate__(state)
         self._plan = None
         self._kept = getattr(self, "_kept", [])
+        self._captured = getattr(self, "_captured", False)
         for held in ("_workspace", "_scalars"):
             self._kept += getattr(self, held, {}).values()
             setattr(self, held, {})
         self.last_grad_norm = None
-        for p, held in self.__dict__.pop("_incoming", ()):
-            self.state[p] = held
+        for p, held, old in self.__dict__.pop("_incoming", ()):
+            self.state[p] = self._in_place(held, old) if self._captured and old else held
+
+    @torch.no_grad()
+    def _in_place(self, held, old):
+        """A loaded state, in the tensors of the old one (whose addresses captured graphs hold) where it is laid out
+        like it."""
+        if held.keys() != old.keys() or any(not torch.is_tensor(t) or t.dtype != held[k].dtype or
+                                            t.device != held[k].device or t.shape != held[k].shape for k, t in old.items()):
+            return held
+        for k, t in old.items():
+            t.copy_(held[k])
+        return old
 
     def add_param_group(self, param_group):
         if isinstance(param_group, dict):
@@ -303,12 +316,13 @@ class _AdamWBase(Optimizer):
                 return None  # torch refuses it
             own = chain.from_iterable(g["params"] for g in self.param_groups)
             names = [(name, g) for g in groups for name in g["params"]]
-            self._incoming = [(p, self._loaded(p, sd["state"][name], group)) for p, (name, group) in zip(own, names)
-                              if sd["state"].get(name)]
+            self._incoming = [(p, self._loaded(p, sd["state"][name], group), self.state.get(p))
+                              for p, (name, group) in zip(own, names) if sd["state"].get(name)]
             # torch's loader would cast every tensor to the parameter's type
             taken = {name for name, _ in names}
             return dict(sd, state={k: v for k, v in sd["state"].items() if k not in taken})
 
+        rates, states = ([g["lr"] for g in self.param_groups], dict(self.state)) if self._captured else ((), {})
         # registered last: sees the dict as the other hooks leave it
         hook = self.register_load_state_dict_pre_hook(prepare)
         try:
@@ -319,6 +333,17 @@ class _AdamWBase(Optimizer):
         for group in self.param_groups:
             for key, value in self.defaults.items():
                 group.setdefault(key, value)
+        # what captured graphs hold stays alive, and a learning rate on the device is theirs still, unless the groups
+        # that share it have come apart
+        self._kept += [st for p, st in states.items() if self.state.get(p) is not st]
+        for lr in {id(lr): lr for lr in rates if torch.is_tensor(lr)}.values():
+            groups = [g for g, r in zip(self.param_groups, rates) if r is lr]
+            if len({float(g["lr"]) for g in groups}) == 1:
+                lr.fill_(float(groups[0]["lr"]))
+                for g in groups:
+                    g["lr"] = lr
+            else:
+                self._kept.append(lr)
 
     def _loaded(self, p, saved, group):
         """A saved state as this optimizer holds it, in tensors of its own."""
@@ -450,6 +475,8 @@ class _AdamWBase(Optimizer):
 
     def _run_plan(self, grad_scale) -> int:
         _, _, cap, index, tensors = self._plan
+        if self.capturable and not self._captured:
+            self._captured = torch.cuda.is_current_stream_capturing()
         scale = self._scale_address(grad_scale, index)
         rc = _host_ext().adamw_run(cap, self._scalar_address(index, tensors), scale, *self._norm_buffers(index, tensors))
         if rc > 0:
@@ -467,6 +494,8 @@ class _AdamWBase(Optimizer):
         one layout: the latter are stepped on contiguous copies, written back in
         stream order."""
         per_dev = {}
+        if self.capturable and not self._captured:
+            self._captured = torch.cuda.is_current_stream_capturing()
         for item in items:
             per_dev.setdefault(item[0].device, []).append(item)
         if len(per_dev) > 1 and (self.max_grad_norm is not None or grad_scale is not None):
@@ -565,7 +594,9 @@ class AdamW(_AdamWBase):
     ``capturable``: the step can be captured into a CUDA graph and replayed.  The
     step counts are then fp32 device tensors and the scalars are formed on the
     device (one more launch); ``lr`` may be an fp32 device tensor, which replays
-    read.  Take a step before the capture: it makes the state.
+    read.  Take a step before the capture: it makes the state.  Graphs hold addresses:
+    after a capture ``load_state_dict`` writes to the states' present tensors, and
+    the optimizer, its parameters and their gradients have to outlive the graphs.
 
     ``state[p]``: ``step`` (int), ``exp_avg``, ``exp_avg_sq``, with master weights
     ``master``."""

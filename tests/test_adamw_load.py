@@ -155,3 +155,65 @@ def test_groups_without_an_option_take_the_optimizers(cls):
         sd["param_groups"][0].pop(key, None)
     opt.load_state_dict(sd)
     _same_state(opt.state_dict(), before)
+
+
+@BOTH
+def test_capturable_loads_write_to_the_states_that_graphs_hold(cls):
+    """A captured step holds the addresses of its states, step counts and learning rate: a load keeps them."""
+    sizes = [30, 5000]
+    opt = cls([_p(n, torch.bfloat16) for n in sizes], lr=torch.tensor(0.25), capturable=True, master_weights=True)
+    sd = opt.state_dict()
+    sd["state"] = {i: dict(_floats(n, i), master=torch.ones(n)) for i, n in enumerate(sizes)}
+    if cls is AdamW8bit:
+        sd["state"][1] = dict(_coded(5000, 128), master=torch.ones(5000))
+    opt.load_state_dict(sd)
+    params = opt.param_groups[0]["params"]
+    held = [dict(opt.state[p]) for p in params]
+    lr = opt.param_groups[0]["lr"]
+    address = [{k: t.data_ptr() for k, t in st.items()} for st in held]
+    opt._captured = True
+    other = copy.deepcopy(opt.state_dict())
+    for st in other["state"].values():
+        for t in st.values():
+            t.copy_(t.flip(0) if t.dim() else t + 5)
+    other["param_groups"][0]["lr"] = torch.tensor(0.125)
+    opt.load_state_dict(copy.deepcopy(other))
+    for i, (p, st, at) in enumerate(zip(params, held, address)):
+        assert opt.state[p].keys() == st.keys()
+        for k, t in st.items():
+            assert opt.state[p][k] is t and t.data_ptr() == at[k] and torch.equal(t, other["state"][i][k]), (i, k)
+    assert opt.param_groups[0]["lr"] is lr and float(lr) == 0.125
+    # a state that cannot stay where it is: the old one stays alive for the graphs
+    gone = opt.state[params[0]]["exp_avg"]
+    changed = copy.deepcopy(other)
+    del changed["state"][0]["master"]
+    opt.load_state_dict(changed)
+    assert "master" not in opt.state[params[0]] and opt.state[params[0]]["exp_avg"] is not gone
+    assert any(isinstance(kept, dict) and kept.get("exp_avg") is gone for kept in opt._kept)
+    gone = opt.state[params[1]]
+    del changed["state"][1]
+    opt.load_state_dict(changed)
+    assert not opt.state[params[1]] and any(kept is gone for kept in opt._kept)
+    # nothing captured: a state dict taken before keeps its tensors
+    plain = cls([_p(30)], capturable=True)
+    plain.load_state_dict({"state": {0: _floats(30)}, "param_groups": plain.state_dict()["param_groups"]})
+    before = plain.state_dict()
+    plain.load_state_dict({"state": {0: _floats(30, 1)}, "param_groups": before["param_groups"]})
+    assert torch.equal(before["state"][0]["exp_avg"], _floats(30)["exp_avg"]) and not plain._kept
+
+
+@BOTH
+def test_a_learning_rate_that_groups_share(cls):
+    lr = torch.tensor(0.5)
+    opt = cls([{"params": [_p(3)]}, {"params": [_p(4)]}, {"params": [_p(5)], "lr": 0.25}], lr=lr, capturable=True)
+    opt._captured = True
+    sd = copy.deepcopy(opt.state_dict())
+    for g in sd["param_groups"][:2]:
+        g["lr"] = torch.tensor(0.125)
+    opt.load_state_dict(sd)
+    assert [g["lr"] is lr for g in opt.param_groups] == [True, True, False] and float(lr) == 0.125
+    assert opt.param_groups[2]["lr"] == 0.25
+    sd["param_groups"][1]["lr"] = torch.tensor(2.0)
+    opt.load_state_dict(sd)
+    assert [float(g["lr"]) for g in opt.param_groups] == [0.125, 2.0, 0.25]
+    assert any(kept is lr for kept in opt._kept)

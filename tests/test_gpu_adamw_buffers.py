@@ -1,5 +1,7 @@
 """AdamW, AdamW8bit and the gradient norm on the GPU give the same bits whatever torch's default dtype is."""
 
+import copy
+
 import numpy as np
 import pytest
 import torch
@@ -49,3 +51,51 @@ def test_the_default_dtype_changes_nothing(cls, default):
     assert len(got) == len(want)
     assert all(a.dtype == b.dtype and torch.equal(a, b) for a, b in zip(got, want))
     assert 1003.0 in [float(t) for t in got if t.dtype == torch.float32 and t.dim() == 0]
+
+
+@pytest.mark.parametrize("cls", [AdamW, AdamW8bit])
+def test_a_load_between_replays_of_a_captured_step(cls):
+    """A graph goes on with the state that was loaded, as eager steps do."""
+    r = np.random.default_rng(1)
+    sizes = [5000, 30, 2049]
+    normal = lambda n, s: torch.from_numpy(r.normal(0, s, n).astype(np.float32)).cuda()  # noqa: E731
+    start = [normal(n, 0.1) for n in sizes]
+    grads = [[normal(n, 1e-2) for n in sizes] for _ in range(6)]
+    kw = dict(capturable=True, max_grad_norm=0.1)
+    lr, lr2 = torch.tensor(1e-2, device="cuda"), torch.tensor(1e-2, device="cuda")
+    params, plain = ([torch.nn.Parameter(t.clone()) for t in start] for _ in range(2))
+    opt, ref = cls(params, lr=lr, **kw), cls(plain, lr=lr2, **kw)
+
+    def set_grads(step):
+        for ps in (params, plain):
+            for p, g in zip(ps, grads[step]):
+                if p.grad is None:
+                    p.grad = g.clone()
+                else:
+                    p.grad.copy_(g)
+
+    set_grads(0)
+    opt.step()
+    ref.step()
+    saved = copy.deepcopy(opt.state_dict())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for step in range(1, 6):
+        set_grads(step)
+        if step == 3:
+            saved["param_groups"][0]["lr"] = torch.tensor(0.5)
+            opt.load_state_dict(saved)
+            ref.load_state_dict(saved)
+            assert opt.param_groups[0]["lr"] is lr and float(lr) == 0.5
+            ref.param_groups[0]["lr"] = torch.tensor(0.5, device="cuda")
+        graph.replay()
+        ref.step()
+        for p, q in zip(params, plain):
+            assert torch.equal(p.detach(), q.detach()), step
+            assert opt.state[p].keys() == ref.state[q].keys()
+            assert all(torch.equal(t, ref.state[q][k]) for k, t in opt.state[p].items()), step
+    assert float(opt.state[params[0]]["step"]) == 4.0
+    opt.step()
+    ref.step()
+    assert all(torch.equal(p.detach(), q.detach()) for p, q in zip(params, plain))
