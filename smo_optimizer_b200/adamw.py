@@ -216,10 +216,11 @@ class _AdamWBase(Optimizer):
         self._plan = None
         self._kept = getattr(self, "_kept", [])
         self._captured = getattr(self, "_captured", False)
-        for held in ("_workspace", "_scalars"):
-            self._kept += getattr(self, held, {}).values()
-            setattr(self, held, {})
-        self.last_grad_norm = None
+        if not self._captured:
+            for held in ("_workspace", "_scalars"):
+                self._kept += getattr(self, held, {}).values()
+                setattr(self, held, {})
+            self.last_grad_norm = None
         for p, held, old in self.__dict__.pop("_incoming", ()):
             self.state[p] = self._in_place(held, old) if self._captured and old else held
 

@@ -217,3 +217,16 @@ def test_a_learning_rate_that_groups_share(cls):
     opt.load_state_dict(sd)
     assert [float(g["lr"]) for g in opt.param_groups] == [0.125, 2.0, 0.25]
     assert any(kept is lr for kept in opt._kept)
+
+
+@BOTH
+def test_a_load_keeps_the_norm_that_graphs_write(cls):
+    opt = cls([_p(3)], capturable=True, max_grad_norm=1.0)
+    norm, scalars = torch.zeros(()), torch.zeros(1, 8)
+    opt._workspace[0], opt._scalars[0], opt.last_grad_norm = (torch.zeros(8), norm), scalars, norm
+    opt._captured = True
+    opt.load_state_dict(opt.state_dict())
+    assert opt.last_grad_norm is norm and opt._workspace[0][1] is norm and opt._scalars[0] is scalars
+    opt._captured = False
+    opt.load_state_dict(opt.state_dict())
+    assert opt.last_grad_norm is None and not opt._workspace and any(kept is scalars for kept in opt._kept)

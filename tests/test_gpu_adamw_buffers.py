@@ -91,6 +91,7 @@ def test_a_load_between_replays_of_a_captured_step(cls):
             ref.param_groups[0]["lr"] = torch.tensor(0.5, device="cuda")
         graph.replay()
         ref.step()
+        assert torch.equal(opt.last_grad_norm, ref.last_grad_norm), step
         for p, q in zip(params, plain):
             assert torch.equal(p.detach(), q.detach()), step
             assert opt.state[p].keys() == ref.state[q].keys()
